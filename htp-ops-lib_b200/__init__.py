@@ -40,7 +40,34 @@ WT_F16_TILED = 1  # fp16 weights in the reference's tile order (HTP_B200_WT_F16_
 WT_PERMUTED = 0x100  # | TYPE_*: the reference-private permuted super-blocks (HTP_B200_WT_PERMUTED)
 ACT_F32 = 0
 ACT_F16 = 1
+KV_I8 = 0  # element codes of an 8-bit key/value cache (HTP_B200_KV_*)
+KV_E4M3 = 1
+ROPE_NONE = 0  # position rotation (HTP_B200_ROPE_*)
+ROPE_PAIRS = 1
+ROPE_HALVES = 2
 BLOCK_BYTES = {TYPE_Q4_0: 18, TYPE_Q8_0: 34, TYPE_IQ4_NL: 18}
+
+class PagedKv(ctypes.Structure):
+    """struct HtpB200PagedKv (include/htp_ops_b200.h)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "k_scale", "v_scale", "page_table", "q_start",
+                                                "ctx_len")]
+                + [(n, ctypes.c_int32) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim", "kv_type", "n_seqs",
+                                                 "table_stride", "n_rows")])
+
+
+class Rope(ctypes.Structure):
+    """struct HtpB200Rope."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("table", "positions")]
+                + [(n, ctypes.c_int32) for n in ("table_len", "rot_dim", "mode")])
+
+
+class LogitsParams(ctypes.Structure):
+    """struct HtpB200LogitsParams."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("history", "history_start", "prompt_len", "repetition", "presence",
+                                                "frequency", "bias_token", "bias_value", "bias_start", "mask",
+                                                "mask_row")]
+                + [(n, ctypes.c_int32) for n in ("n_history", "n_bias", "n_mask_rows")])
+
 
 # every symbol include/*.h declares, with (restype, argtypes)
 _vp, _i, _u, _sz, _i64, _u64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_uint, ctypes.c_size_t, ctypes.c_int64,
@@ -59,6 +86,12 @@ EXPORTS = {
     "htp_b200_mul_mat_gather_step": (_i, [_vp, _i, _i64, _i64, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, ctypes.c_uint32,
                                           _vp]),
     "htp_b200_wait_flags": (_i, [_vp, _i, ctypes.c_uint32, _vp]),
+    "htp_b200_kv_append": (_i, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _i, _i, _vp]),
+    "htp_b200_attn_paged": (_i, [_vp, _i64, _vp, _i64, _vp, _i, _i, ctypes.c_float, _i, _i, _i, _vp, _sz, _vp]),
+    "htp_b200_attn_workspace": (_sz, [_vp, _i, _i, _i, _i]),
+    "htp_b200_add_rms_norm": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, ctypes.c_float, ctypes.c_float, _i, _i, _i,
+                                   _vp]),
+    "htp_b200_logits_process": (_i, [_vp, _vp, _i64, _i, _i, _vp, _vp]),
     "htp_b200_weight_bytes": (_sz, [_i, _i64, _i64]),
     "htp_b200_stream_status": (_i, [_vp]),
     "htp_b200_set_option": (_i, [ctypes.c_char_p, _i]),

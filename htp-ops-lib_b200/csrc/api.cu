@@ -874,7 +874,8 @@ int htp_b200_stream_status(void *stream) {
     cudaMemsetAsync(sc->counters, 0, (size_t) kGemvMaxGrid * sizeof(unsigned), st);
     cudaStreamSynchronize(st);
   }
-  return code;
+  const int device_code = take_device_error(ctx);
+  return code != 0 ? code : device_code;
 }
 
 int htp_b200_set_option(const char *name, int value) {

@@ -1,0 +1,665 @@
+// Attention over the paged 8-bit cache for few rows per sequence (formula: include/htp_ops_b200.h,
+// htp_b200_attn_paged).
+//
+// All query rows and heads that read one key/value head are the COLUMNS of one tile (8 or 16 of them), so
+// every code is fetched from HBM once and the warp-level tensor-core instructions work on full tiles:
+//   S^T[token][column] = K[token][d] . Q^T[d][column]     A = 16 tokens of codes, B = the queries
+//   O^T[d][column]    += V^T[d][token] . P^T[token][column]
+// Codes become fp16 exactly (signed bytes and e4m3 both fit) on their way from global memory to the A
+// fragments, in registers: the order of d inside a fragment is free as long as K and Q (or V^T and O^T)
+// agree, so each lane loads 16 contiguous bytes of a row.  P^T comes from S^T by an 8 x 8 transpose in the
+// warp.  fp32 queries and weights are two fp16 terms each (hi + lo), two MMAs into the same accumulator.
+//
+// Scales never touch the codes.  With x = s * (k_scale * scale * log2 e) + log2(v_scale) the weight
+// n = 2^(x - M) carries the value block's scale (M: running maximum of x, raised only when x leaves it more
+// than kSlack behind), O sums n * code, and the softmax denominator sums n / v_scale per block: one running
+// maximum, one FMA and one exponential per score, everything in fp32.
+//
+// Work: CTA = 4 warps; a warp walks 32-token steps of its CTA's share of the context, its next loads issued
+// while the current step computes.  A context is shared by the CTAs of a cluster, whose results meet in
+// distributed shared memory in rank order; long contexts of few sequences by several clusters, whose results
+// meet in the workspace and a second small launch.  No atomics: results do not depend on scheduling.
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "decoder_common.cuh"
+#include "ptx.cuh"
+#include "unpack.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace htp {
+
+namespace {
+
+constexpr int   kWarps   = 4;
+constexpr int   kThreads = kWarps * 32;
+constexpr int   kStep    = 32;     // tokens of a warp's step: two 16-token MMA tiles
+constexpr float kLift    = 8.f;    // weights are kept times 2^8: fp16 terms of small weights stay normal numbers
+constexpr float kSlack   = 6.f;    // M may lag the maximum by this much: weights stay below 2^(8 + 6) < 65504
+constexpr float kFloor   = -1e30f; // M before the first score
+
+// Four codes (lowest byte first) as two fp16 pairs.
+template <int KVT>
+__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t (&h)[2]) {
+  if constexpr (KVT == kKvI8) {
+    q8_0_unpack_word(w, h);
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w & 0xffff), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w >> 16), __NV_E4M3);
+    h[0]                = (uint32_t) a.x | (uint32_t) a.y << 16;
+    h[1]                = (uint32_t) b.x | (uint32_t) b.y << 16;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  return h2_as_u32(__floats2half2_rn(a, b));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// hi + lo fp16 terms of two fp32 values
+__device__ __forceinline__ void split_h2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2  f = __half22float2(h);
+  hi              = h2_as_u32(h);
+  lo              = pack_h2(a - f.x, b - f.y);
+}
+
+// The weight of a score.  Scores so large that their rounding exceeds kSlack stay finite; NaN stays NaN.
+__device__ __forceinline__ float weight_of(float y) {
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(kLift + kSlack));
+  return exp2_approx(y);
+}
+
+template <int KVT, int D, int NT, bool F32>
+__global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int NC    = NT * 8;
+  constexpr int KI    = D / 64;          // 16-byte pieces of a key row per lane
+  constexpr int MT    = D / 16;          // 16-row tiles of O^T
+  constexpr int VW    = D / 32;          // words of a value row per lane (8 lanes x VW words = a row)
+  constexpr int TERMS = F32 ? 2 : 1;
+  constexpr int QP    = D + 8;           // pitch of a query column in shared memory (halves): conflict-free 16-byte reads
+  constexpr int OP    = D + 4;           // pitch of an output column (floats)
+  __shared__ __align__(16) union {
+    __half q[TERMS][NC][QP];
+    float  o[kWarps][NC][OP];
+  } sm;
+  __shared__ float ml[kWarps][2][NC];
+  __shared__ float q_unit[NC];  // fp32 queries: the power of two that a column was divided by
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+
+  const KvView &kv   = a.kv;
+  const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned      id    = blockIdx.x;
+  const int     split = id % a.splits;
+  id /= a.splits;
+  const int grp = id % a.groups;
+  id /= a.groups;
+  const int head = id % kv.n_kv_heads;
+  id /= kv.n_kv_heads;
+  const int cols0 = (int) (id % a.col_groups) * NC;
+  const int b     = id / a.col_groups;
+
+  int q0, q_len, ctx;
+  if (!sequence_of(kv, b, a.max_q, a.max_ctx, q0, q_len, ctx)) {
+    if (threadIdx.x == 0) {
+      record_error(a.err, kErrSequence);
+    }
+    return;  // (every CTA of the cluster leaves here)
+  }
+  const int n_cols = q_len * a.group - cols0 < NC ? q_len * a.group - cols0 : NC;  // columns in use
+  if (n_cols <= 0) {
+    return;
+  }
+  const int past = ctx - q_len;  // token number of row 0 (negative: the first rows see nothing)
+  const int r0 = cols0 / a.group, r1 = (cols0 + n_cols - 1) / a.group;
+  int       hi = past + r1 + 1, lo = 0;
+  hi = hi < 0 ? 0 : hi;
+  if (a.window > 0 && past + r0 - a.window + 1 > 0) {
+    lo = past + r0 - a.window + 1;
+  }
+  const int s0 = lo / kStep, steps = hi > lo ? (hi + kStep - 1) / kStep - s0 : 0;
+  const int parts = a.splits * a.groups, part = grp * a.splits + split;
+  const int begin = s0 + (int) ((long long) steps * part / parts), end = s0 + (int) ((long long) steps * (part + 1) / parts);
+
+  // queries -> shared memory, unused columns as zeros.  fp32 columns are divided by the power of two that
+  // brings their largest magnitude into [2^13, 2^14): nothing overflows fp16 and the second term keeps its bits.
+  for (int i = threadIdx.x; i < NC * (D / 4); i += kThreads) {
+    const int c = i / (D / 4), d = i % (D / 4) * 4;
+    float4    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < n_cols) {
+      const int       r  = (cols0 + c) / a.group, h = head * a.group + (cols0 + c) % a.group;
+      const long long at = (long long) (q0 + r) * a.q_stride + h * D + d;
+      if constexpr (F32) {
+        v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
+      } else {
+        *reinterpret_cast<uint2 *>(&sm.q[0][c][d]) = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + at);
+        continue;
+      }
+    }
+    if constexpr (F32) {
+      float m = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+      for (int o = D / 8; o > 0; o >>= 1) {  // (the D / 4 lanes of a column: a warp, or half of one)
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
+      int e = ((__float_as_int(m) >> 23) & 0xff) - 127 - 13;
+      e     = m == 0.f ? 0 : (e < -100 ? -100 : e);
+      const float f = __int_as_float((127 - e) << 23);
+      v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+      if (d == 0) {
+        q_unit[c] = __int_as_float((127 + e) << 23);
+      }
+    }
+    uint2 h, l;
+    split_h2(v.x, v.y, h.x, l.x);
+    split_h2(v.z, v.w, h.y, l.y);
+    *reinterpret_cast<uint2 *>(&sm.q[0][c][d]) = h;
+    if constexpr (F32) {
+      *reinterpret_cast<uint2 *>(&sm.q[TERMS - 1][c][d]) = l;
+    }
+  }
+  // what the lane's columns (2 t, 2 t + 1 of each 8) see: tokens first[] .. last[]
+  int last[NT][2], first[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = cols0 + n * 8 + 2 * t + j;
+      last[n][j]  = past + c / a.group;
+      first[n][j] = a.window > 0 ? last[n][j] - a.window + 1 : 0;
+    }
+  }
+  const int all_from = a.window > 0 ? past + r1 - a.window + 1 : 0, all_to = past + r0;  // seen by every column
+
+  const int       P = kv.page_size;
+  const int      *table = kv.page_table + (long long) b * kv.table_stride;
+  // page of a step's tile, -1 where there is nothing to read (outside lo .. hi, or a bad entry)
+  auto page_of = [&](int step, int tile) {
+    const int tok = step * kStep + tile * 16;
+    if (step >= end || tok >= hi || tok + 16 <= lo) {
+      return -1;
+    }
+    const int p = table[tok >> kv.page_shift];
+    if (p < 0 || p >= kv.n_pages) {
+      if (lane == 0) {
+        record_error(a.err, kErrPage);
+      }
+      return -1;
+    }
+    return p;
+  };
+  uint4    kr[2][2][KI];
+  uint32_t vr[2][4][VW];
+  float    ks[2], vs[2];
+  auto     offset = [&](int page, int step, int tile) {
+    return ((((long long) page * kv.n_kv_heads + head) << kv.page_shift) + ((step * kStep + tile * 16) & (P - 1))) * D;
+  };
+  auto load_k = [&](int step, const int (&pg)[2]) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (pg[m] >= 0) {
+        const uint8_t *base = kv.k_codes + offset(pg[m], step, m) + g * D + t * 16;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int i = 0; i < KI; ++i) {
+            kr[m][r][i] = ld_stream16(base + r * 8 * D + i * 64);
+          }
+        }
+        ks[m] = kv.k_scale[(long long) pg[m] * kv.n_kv_heads + head];
+      }
+    }
+  };
+  auto load_v = [&](int step, const int (&pg)[2]) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      if (pg[m] >= 0) {
+        const uint8_t *base = kv.v_codes + offset(pg[m], step, m) + g * (D / 8);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+          const uint8_t *at = base + (2 * t + (r & 1) + (r >> 1) * 8) * D;
+          if constexpr (VW == 4) {
+            const uint4 v = ld_stream16(at);
+            vr[m][r][0] = v.x, vr[m][r][1] = v.y, vr[m][r][2] = v.z, vr[m][r][3] = v.w;
+          } else {
+            const uint2 v = ld_stream8(at);
+            vr[m][r][0] = v.x, vr[m][r][1] = v.y;
+          }
+        }
+        vs[m] = kv.v_scale[(long long) pg[m] * kv.n_kv_heads + head];
+      }
+    }
+  };
+
+  float o[NT][MT][4], l[NT][2], mx[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    l[n][0] = l[n][1] = 0.f;
+    mx[n][0] = mx[n][1] = kFloor;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+    }
+  }
+  int pg[2], pn[2];
+  int step = begin + warp;
+  pg[0] = page_of(step, 0), pg[1] = page_of(step, 1);
+  load_k(step, pg);
+  load_v(step, pg);
+  pn[0] = page_of(step + kWarps, 0), pn[1] = page_of(step + kWarps, 1);
+  __syncthreads();  // the queries are in place
+  float unit[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unit[n][j] = F32 ? q_unit[n * 8 + 2 * t + j] : 1.f;
+    }
+  }
+
+  for (; step < end; step += kWarps) {
+    // ---- scores
+    float s[2][NT][4];
+    float by[2], up[2], inv[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float v = vs[m] > 0.f ? vs[m] : 1.f;
+      by[m]         = pg[m] >= 0 && ks[m] > 0.f ? ks[m] * a.scale_log2 : a.scale_log2;
+      up[m]         = pg[m] >= 0 ? log2f(v) : 0.f;
+      inv[m]        = pg[m] >= 0 ? 1.f / v : 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+#pragma unroll
+      for (int w2 = 0; w2 < 2; ++w2) {
+        uint4 qf[NT][TERMS];  // two words of codes against 8 halves of the lane's column
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int x = 0; x < TERMS; ++x) {
+            qf[n][x] = *reinterpret_cast<const uint4 *>(&sm.q[x][n * 8 + g][i * 64 + t * 16 + w2 * 8]);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int w1 = 0; w1 < 2; ++w1) {
+            const uint32_t c0 = w2 ? (w1 ? kr[m][0][i].w : kr[m][0][i].z) : (w1 ? kr[m][0][i].y : kr[m][0][i].x);
+            const uint32_t c1 = w2 ? (w1 ? kr[m][1][i].w : kr[m][1][i].z) : (w1 ? kr[m][1][i].y : kr[m][1][i].x);
+            uint32_t       h0[2], h1[2];
+            codes_to_h2<KVT>(c0, h0);
+            codes_to_h2<KVT>(c1, h1);
+            const uint32_t af[4] = { h0[0], h1[0], h0[1], h1[1] };
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+              for (int x = 0; x < TERMS; ++x) {
+                mma_16816(s[m][n], af, w1 ? qf[n][x].z : qf[n][x].x, w1 ? qf[n][x].w : qf[n][x].y);
+              }
+            }
+          }
+        }
+      }
+    }
+    const bool next = step + kWarps < end;
+    const int  live[2] = { pg[0], pg[1] };
+    if (next) {
+      load_k(step + kWarps, pn);
+    }
+    // ---- weights
+    const int  tok0 = step * kStep;
+    const bool full = live[0] >= 0 && live[1] >= 0 && tok0 >= all_from && tok0 + kStep - 1 <= all_to;
+    if (!full) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int tok = tok0 + m * 16 + g + (e >> 1) * 8;
+            if (live[m] < 0 || tok > last[n][e & 1] || tok < first[n][e & 1]) {
+              s[m][n][e] = -INFINITY;
+            }
+          }
+        }
+      }
+    }
+    float y[2][NT][4];
+    float top = -INFINITY;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[m][n][e] = fmaf(s[m][n][e], by[m] * unit[n][e & 1], up[m] - mx[n][e & 1] + kLift);
+          top        = fmaxf(top, y[m][n][e]);
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, top > kLift + kSlack)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float x = kFloor;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            x = fmaxf(x, fmaxf(fmaf(s[m][n][j], by[m] * unit[n][j], up[m]), fmaf(s[m][n][j + 2], by[m] * unit[n][j], up[m])));
+          }
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          x = fmaxf(x, mx[n][j]);
+          const float f = exp2_approx(mx[n][j] - x);
+          mx[n][j]      = x;
+          l[n][j] *= f;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[n][i][j] *= f;
+            o[n][i][j + 2] *= f;
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            y[m][n][e] = fmaf(s[m][n][e], by[m] * unit[n][e & 1], up[m] - mx[n][e & 1] + kLift);
+          }
+        }
+      }
+    }
+    uint32_t pf[2][NT][TERMS][2];  // B fragments: tokens 2 t, 2 t + 1 and 2 t + 8, 2 t + 9 of column g
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[m][n][e] = weight_of(y[m][n][e]);
+        }
+        l[n][0] = fmaf(y[m][n][0] + y[m][n][2], inv[m], l[n][0]);
+        l[n][1] = fmaf(y[m][n][1] + y[m][n][3], inv[m], l[n][1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          if constexpr (F32) {
+            uint32_t h, lo16;
+            split_h2(y[m][n][2 * r], y[m][n][2 * r + 1], h, lo16);
+            pf[m][n][0][r]         = transpose8x8(h);
+            pf[m][n][TERMS - 1][r] = transpose8x8(lo16);
+          } else {
+            pf[m][n][0][r] = transpose8x8(pack_h2(y[m][n][2 * r], y[m][n][2 * r + 1]));
+          }
+        }
+      }
+    }
+    // ---- O^T += V^T P^T
+    // (codes behind the context may be no numbers: their weight 0 would not hide them)
+    if (!full) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int tok = tok0 + m * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
+          if (live[m] < 0 || tok >= hi || tok < lo) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              vr[m][r][w] = 0;
+            }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // codes (token A, token B) of d = 4 w + 2 half and of the one after it, side by side
+          const uint32_t sel = half ? 0x7362 : 0x5140;
+          uint32_t       ab[2], cd[2];
+          codes_to_h2<KVT>(__byte_perm(vr[m][0][w], vr[m][1][w], sel), ab);
+          codes_to_h2<KVT>(__byte_perm(vr[m][2][w], vr[m][3][w], sel), cd);
+          const uint32_t af[4] = { ab[0], ab[1], cd[0], cd[1] };
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) {
+              mma_16816(o[n][2 * w + half], af, pf[m][n][x][0], pf[m][n][x][1]);
+            }
+          }
+        }
+      }
+    }
+    if (next) {
+      load_v(step + kWarps, pn);
+      pg[0] = pn[0], pg[1] = pn[1];
+      pn[0] = page_of(step + 2 * kWarps, 0), pn[1] = page_of(step + 2 * kWarps, 1);
+    }
+  }
+
+  // ---- the warps' results, in warp order
+  __syncthreads();  // the queries are no longer needed
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = n * 8 + 2 * t + j;
+      float     x = l[n][j];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (g == 0) {
+        ml[warp][0][c] = mx[n][j];
+        ml[warp][1][c] = x;
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        *reinterpret_cast<float2 *>(&sm.o[warp][c][g * (D / 8) + 2 * i]) = make_float2(o[n][i][j], o[n][i][j + 2]);
+      }
+    }
+  }
+  __syncthreads();
+  constexpr int PER = NC * (D / 4) / kThreads;  // groups of four outputs a thread adds
+  float         m_cta[PER], l_cta[PER];
+  float4        acc[PER];
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int i = threadIdx.x + p * kThreads, c = i / (D / 4), d = i % (D / 4) * 4;
+    float     m = kFloor, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      m = fmaxf(m, ml[w][0][c]);
+    }
+    acc[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float  f = exp2_approx(ml[w][0][c] - m);
+      const float4 v = *reinterpret_cast<const float4 *>(&sm.o[w][c][d]);
+      sum            = fmaf(f, ml[w][1][c], sum);
+      acc[p].x = fmaf(f, v.x, acc[p].x), acc[p].y = fmaf(f, v.y, acc[p].y);
+      acc[p].z = fmaf(f, v.z, acc[p].z), acc[p].w = fmaf(f, v.w, acc[p].w);
+    }
+    m_cta[p] = m, l_cta[p] = sum;
+  }
+
+  // ---- the cluster's results, in rank order: every CTA leaves its sums in warp slot 0, then each thread of
+  // rank r adds the groups i with i % splits == r
+  if (a.splits > 1) {
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * kThreads, c = i / (D / 4), d = i % (D / 4) * 4;
+      *reinterpret_cast<float4 *>(&sm.o[0][c][d]) = acc[p];
+      if (d == 0) {
+        ml[0][0][c] = m_cta[p], ml[0][1][c] = l_cta[p];
+      }
+    }
+    cg::this_cluster().sync();
+  }
+  auto finish = [&](int c, int d, float m, float sum, float4 v) {
+    if (c >= n_cols) {
+      return;
+    }
+    const int r = (cols0 + c) / a.group, h = head * a.group + (cols0 + c) % a.group;
+    if (a.groups > 1) {
+      // partial results, [cluster][sequence][row][head]: D sums, then maximum and denominator
+      const long long at = (((long long) grp * kv.n_seqs + b) * a.max_q + r) * a.n_heads + h;
+      float          *to = a.part + at * (D + 4);
+      *reinterpret_cast<float4 *>(to + d) = v;
+      if (d == 0) {
+        *reinterpret_cast<float2 *>(to + D) = make_float2(m, sum);
+      }
+      return;
+    }
+    const float     f  = sum > 0.f ? 1.f / sum : 0.f;
+    const long long at = (long long) (q0 + r) * a.out_stride + h * D + d;
+    if constexpr (F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+    } else {
+      uint2 u;
+      u.x = pack_h2(v.x * f, v.y * f);
+      u.y = pack_h2(v.z * f, v.w * f);
+      *reinterpret_cast<uint2 *>(static_cast<__half *>(a.out) + at) = u;
+    }
+  };
+  if (a.splits == 1) {
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + p * kThreads;
+      finish(i / (D / 4), i % (D / 4) * 4, m_cta[p], l_cta[p], acc[p]);
+    }
+    return;
+  }
+  cg::cluster_group cluster = cg::this_cluster();
+  for (int i = threadIdx.x * a.splits + split; i < NC * (D / 4); i += kThreads * a.splits) {
+    const int c = i / (D / 4), d = i % (D / 4) * 4;
+    float     m = kFloor, sum = 0.f;
+    float4    v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < a.splits; ++r) {
+      m = fmaxf(m, *cluster.map_shared_rank(&ml[0][0][c], r));
+    }
+    for (int r = 0; r < a.splits; ++r) {
+      const float  f = exp2_approx(*cluster.map_shared_rank(&ml[0][0][c], r) - m);
+      const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sm.o[0][c][d], r));
+      sum            = fmaf(f, *cluster.map_shared_rank(&ml[0][1][c], r), sum);
+      v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+    }
+    finish(c, d, m, sum, v);
+  }
+  cluster.sync();  // nobody leaves while others read its shared memory
+}
+
+// The clusters' results of one (sequence, row, head) per warp, in cluster order.
+template <int D, bool F32>
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs a) {
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+  const long long id   = (long long) blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int       lane = threadIdx.x & 31;
+  const int       h = (int) (id % a.n_heads), r = (int) (id / a.n_heads % a.max_q), b = (int) (id / a.n_heads / a.max_q);
+  int             q0, q_len, ctx;
+  if (b >= a.kv.n_seqs || !sequence_of(a.kv, b, a.max_q, a.max_ctx, q0, q_len, ctx) || r >= q_len) {
+    return;
+  }
+  const long long each = (long long) a.kv.n_seqs * a.max_q * a.n_heads * (D + 4);
+  const float    *from = a.part + id * (D + 4);
+  float           m = kFloor, sum = 0.f, v[D / 32] = {};
+  for (int k = 0; k < a.groups; ++k) {
+    m = fmaxf(m, from[k * each + D]);
+  }
+  for (int k = 0; k < a.groups; ++k) {
+    const float f = exp2_approx(from[k * each + D] - m);
+    sum           = fmaf(f, from[k * each + D + 1], sum);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      v[i] = fmaf(f, from[k * each + lane * (D / 32) + i], v[i]);
+    }
+  }
+  const float     f  = sum > 0.f ? 1.f / sum : 0.f;
+  const long long at = (long long) (q0 + r) * a.out_stride + h * D + lane * (D / 32);
+#pragma unroll
+  for (int i = 0; i < D / 32; i += 2) {
+    if constexpr (F32) {
+      *reinterpret_cast<float2 *>(static_cast<float *>(a.out) + at + i) = make_float2(v[i] * f, v[i + 1] * f);
+    } else {
+      *reinterpret_cast<uint32_t *>(static_cast<__half *>(a.out) + at + i) = pack_h2(v[i] * f, v[i + 1] * f);
+    }
+  }
+}
+
+template <int KVT, int D, bool F32>
+cudaError_t launch_tiles(const AttnArgs &a, const AttnPlan &p, bool pdl, cudaStream_t st) {
+  const long long grid = (long long) a.kv.n_seqs * p.col_groups * a.kv.n_kv_heads * p.groups * p.splits;
+  if (grid > 0x7fffffffll) {
+    return cudaErrorInvalidConfiguration;
+  }
+  cudaError_t e = p.col_tiles == 1
+                    ? launch_decoder_kernel(attn_decode_kernel<KVT, D, 1, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st)
+                    : launch_decoder_kernel(attn_decode_kernel<KVT, D, 2, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st);
+  if (e == cudaSuccess && p.groups > 1) {
+    const long long rows = (long long) a.kv.n_seqs * a.max_q * a.n_heads;
+    e = launch_decoder_kernel(attn_join_kernel<D, F32>, a, (unsigned) ((rows + 3) / 4), 128, 0, pdl, 1, st);
+  }
+  return e;
+}
+
+}  // namespace
+
+size_t attn_part_bytes(int n_seqs, int max_q, int n_heads, int head_dim, int groups) {
+  return groups > 1 ? (size_t) groups * n_seqs * max_q * n_heads * (head_dim + 4) * sizeof(float) : 0;
+}
+
+AttnPlan attn_plan(int sm_count, int n_seqs, int n_rows, int n_kv_heads, int group, bool f32, int max_q, int max_ctx,
+                   size_t workspace_bytes, int head_dim) {
+  AttnPlan        p    = {};
+  const long long cols = (long long) max_q * group;
+  p.col_tiles          = cols > 8 ? 2 : 1;
+  p.col_groups         = (int) ((cols + 8 * p.col_tiles - 1) / (8 * p.col_tiles));
+  // enough CTAs for about four on every SM, none with less than a step per warp
+  const long long jobs = (long long) n_seqs * n_kv_heads * p.col_groups, want = 4ll * sm_count;
+  const long long most = ((long long) max_ctx + kStep * kWarps - 1) / (kStep * kWarps);
+  p.splits             = 1;
+  while (p.splits < 8 && jobs * p.splits < want && p.splits < most) {
+    p.splits *= 2;
+  }
+  // several clusters over one context: when each still has a few thousand tokens of its own
+  p.groups = 1;
+  while (p.splits == 8 && p.groups < 16 && jobs * 8 * p.groups < want && (long long) max_ctx / (2 * p.groups) >= 4096) {
+    p.groups *= 2;
+  }
+  while (p.groups > 1 && attn_part_bytes(n_seqs, max_q, n_kv_heads * group, head_dim, p.groups) > workspace_bytes) {
+    p.groups /= 2;
+  }
+  (void) n_rows, (void) f32;
+  return p;
+}
+
+cudaError_t attn_decode_launch(const AttnArgs &a, const AttnPlan &p, int head_dim, int kv_type, bool a16, bool pdl,
+                               cudaStream_t st) {
+  if (head_dim == 64) {
+    if (kv_type == kKvI8) {
+      return a16 ? launch_tiles<kKvI8, 64, false>(a, p, pdl, st) : launch_tiles<kKvI8, 64, true>(a, p, pdl, st);
+    }
+    return a16 ? launch_tiles<kKvE4m3, 64, false>(a, p, pdl, st) : launch_tiles<kKvE4m3, 64, true>(a, p, pdl, st);
+  }
+  if (kv_type == kKvI8) {
+    return a16 ? launch_tiles<kKvI8, 128, false>(a, p, pdl, st) : launch_tiles<kKvI8, 128, true>(a, p, pdl, st);
+  }
+  return a16 ? launch_tiles<kKvE4m3, 128, false>(a, p, pdl, st) : launch_tiles<kKvE4m3, 128, true>(a, p, pdl, st);
+}
+
+}  // namespace htp

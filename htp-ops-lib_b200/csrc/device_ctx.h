@@ -31,6 +31,13 @@ DeviceCtx *current_device_ctx();
 // Scratch bound to (current device, stream); allocated on first use.  nullptr on failure.
 StreamScratch *stream_scratch(DeviceCtx *ctx, cudaStream_t stream);
 
+// Word that the operators on paged caches and on logits record errors in, one per device (decoder_ops.cu):
+// host memory that the device addresses, made on first use - also while a stream is being captured - and kept
+// until the process ends (captured graphs hold its address).  nullptr on failure.
+int *device_error_word(DeviceCtx *ctx);
+// Its code, cleared; 0 when there is none.
+int take_device_error(DeviceCtx *ctx);
+
 // Frees every scratch area (used at session close).
 void release_all_scratch();
 

@@ -177,8 +177,144 @@ int htp_b200_wait_flags(const uint32_t *flags, int n, uint32_t epoch, void *stre
  * rules (non-null, non-zero sizes, 128-byte aligned pointers -> else -1), device pointers + stream. */
 int htp_b200_rms_norm_f32(float *dst, const float *src, int ne0, int ne1, void *stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The operators around a decoder's matmuls: a paged key/value cache held in 8 bits (append, attention),
+ * residual and norms, logits processing.  No counterpart in the reference, except that attention does the
+ * work of its FlashAttention operator (include/op_reg.h:36-47) on another cache.  Common rules:
+ *   - they allocate nothing, keep nothing between calls and can be captured into a graph at any time, the
+ *     first call on a stream included;
+ *   - lengths, tables and positions are device memory and are read by the kernels, so a captured call
+ *     follows their contents.  What they say is checked there: an entry out of its range is skipped (no
+ *     access outside the buffers is made, what it covers is left unwritten) and recorded as an error code
+ *     301 .. 305 that the next htp_b200_stream_status of this device returns;
+ *   - host-side checks answer -1 before anything is launched.
+ */
+
+/* element codes of a cache */
+#define HTP_B200_KV_I8 0   /* signed bytes, -127 .. 127 */
+#define HTP_B200_KV_E4M3 1 /* 8-bit floating point, 4 exponent and 3 mantissa bits, up to 448 */
+
+/* A paged cache and the sequences of one step.  A page holds page_size consecutive tokens of one sequence
+ * for every key/value head: codes[page][head][token][head_dim], one scale per page and head; the value
+ * that a code stands for is code * scale.  Sequence b owns rows q_start[b] .. q_start[b + 1] - 1 of the
+ * step's row-major inputs; they are the last tokens of its ctx_len[b] (these rows among them), and token j
+ * lies in page page_table[b][j / page_size].  Rows from q_start[n_seqs] on belong to nobody: they are
+ * neither read nor written.  Entries of the table behind a sequence's last page are not read.  Scales are
+ * positive (0 is taken as 1, for blocks whose codes are all 0); the scales of the value pages one row
+ * attends to lie within a factor of 2^110 of each other. */
+struct HtpB200PagedKv {
+  void          *k_codes;    /* 16-byte aligned, [n_pages][n_kv_heads][page_size][head_dim] bytes */
+  void          *v_codes;
+  float         *k_scale;    /* [n_pages][n_kv_heads] */
+  float         *v_scale;
+  const int32_t *page_table; /* [n_seqs][table_stride] */
+  const int32_t *q_start;    /* [n_seqs + 1], not decreasing, within 0 .. n_rows */
+  const int32_t *ctx_len;    /* [n_seqs] */
+  int32_t        n_pages;
+  int32_t        page_size;  /* 16, 32, 64 or 128 */
+  int32_t        n_kv_heads;
+  int32_t        head_dim;   /* 64 or 128 */
+  int32_t        kv_type;    /* HTP_B200_KV_* */
+  int32_t        n_seqs;
+  int32_t        table_stride;
+  int32_t        n_rows;     /* rows of the step's buffers */
+};
+
+/* Position rotation: of the first rot_dim elements of a head, pairs (a, b) become
+ * (a * cos - b * sin, b * cos + a * sin). */
+#define HTP_B200_ROPE_NONE 0
+#define HTP_B200_ROPE_PAIRS 1  /* pair i = elements 2 i, 2 i + 1 */
+#define HTP_B200_ROPE_HALVES 2 /* pair i = elements i, i + rot_dim / 2 */
+struct HtpB200Rope {
+  const float   *table;     /* [table_len][rot_dim]: the cosines of a position's rot_dim / 2 angles, then the sines */
+  const int32_t *positions; /* [n_rows], or NULL: a row's position is its token number in the sequence */
+  int32_t        table_len;
+  int32_t        rot_dim;   /* a multiple of 8, at most head_dim */
+  int32_t        mode;      /* HTP_B200_ROPE_* */
+};
+
+/* Appends the step's keys and values (rows of n_kv_heads * head_dim elements of act_type) to the cache,
+ * the keys rotated, and writes the rotated queries (rows of n_heads * head_dim) to q_out in q_out_type
+ * (HTP_B200_ACT_*; q = NULL: no queries).  rope = NULL or HTP_B200_ROPE_NONE: no rotation.  Strides count
+ * elements between rows, so q, k and v may be column bands of one matrix; q_out may be q when the types
+ * are the same, and otherwise overlaps nothing.
+ * Scales: with amax the largest finite magnitude of the new elements of a page and head,
+ *   needed = max(amax / 127 (signed bytes) or amax / 448 (e4m3), 2^-100),
+ *   scale  = needed when the page holds no older tokens of the sequence, else max(its scale, needed);
+ * codes of older tokens follow a grown scale: c becomes round(c * (old scale / scale)); new codes are
+ * round(x * (1 / scale)), ties to even, saturated (NaN: 0 in signed bytes, NaN in e4m3).  Every step is a
+ * correctly rounded fp32 operation (products and sums not contracted), so the bytes are reproducible.
+ * Appending the same rows twice gives the same cache as once.  A page that is appended to belongs to one
+ * sequence, once: two that share it may only read it. */
+int htp_b200_kv_append(const struct HtpB200PagedKv *kv, const struct HtpB200Rope *rope, const void *k, int64_t k_stride,
+                       const void *v, int64_t v_stride, const void *q, int64_t q_stride, void *q_out,
+                       int64_t q_out_stride, int n_heads, int act_type, int q_out_type, void *stream);
+
+/* out[row][head] = sum_j softmax_j(scale * q[row][head] . key_j) * value_j over the tokens j that the row
+ * sees: j <= its token number and, with window > 0, j > its token number - window; a row that sees none
+ * gives zeros.  n_heads is a multiple of n_kv_heads, query head i reads key/value head
+ * i / (n_heads / n_kv_heads).  out and q have act_type; fp32 queries and weights go through the
+ * tensor cores as two fp16 terms each, so that fp32 results keep fp32 accuracy.
+ * max_q / max_ctx bound every sequence's rows / context in this call (a sequence over one of them is
+ * skipped, error 302); they choose the kernel and its splits and do not change with the contents of a
+ * captured call.  workspace: htp_b200_attn_workspace bytes of device memory, 16-byte aligned, contents of
+ * no matter, owned by this call until it has finished (two calls that may run at the same time need one
+ * each); with less (or NULL) long contexts of few sequences are read by fewer SMs.  q 16-byte aligned,
+ * strides multiples of 16 bytes; out overlaps none of the inputs. */
+int htp_b200_attn_paged(void *out, int64_t out_stride, const void *q, int64_t q_stride, const struct HtpB200PagedKv *kv,
+                        int n_heads, int act_type, float scale, int window, int max_q, int max_ctx, void *workspace,
+                        size_t workspace_bytes, void *stream);
+/* Bytes of workspace with which htp_b200_attn_paged runs this step at its full speed (0: it needs none).
+ * Host arithmetic on kv's sizes; its pointers are not used.  (size_t) -1 for arguments that
+ * htp_b200_attn_paged rejects. */
+size_t htp_b200_attn_workspace(const struct HtpB200PagedKv *kv, int n_heads, int act_type, int max_q, int max_ctx);
+
+/* What lies between two blocks of a decoder, on rows of n elements:
+ *   b    = block, normed if post_weight is given: b / sqrt(mean(b^2) + eps) * post_weight[n]
+ *   b   *= gate (NULL: none; rows gate_stride elements apart, 0: one row for all)
+ *   h    = x + block_scale * b
+ *   norm = h / sqrt(mean(h^2) + eps) * weight[n] (NULL: 1)
+ * h_out or norm_out may be NULL (not wanted), block too (h = x, the input norm of a first block).  fp32
+ * except norm_out, which norm_type (HTP_B200_ACT_*) makes fp32 or fp16: the activations of the next
+ * matmul.  Rows lie n elements apart.  h_out may be x or block, an fp32 norm_out too (not h_out); other
+ * overlaps are rejected.  Pointers have the alignment of their type; 16-byte aligned ones with n % 4 == 0
+ * (and gate_stride % 4 == 0) are faster. */
+int htp_b200_add_rms_norm(float *h_out, void *norm_out, const float *x, const float *block, const float *post_weight,
+                          const float *gate, int64_t gate_stride, const float *weight, float block_scale, float eps,
+                          int n, int rows, int norm_type, void *stream);
+
+/* What is done to a row's logits before a token is chosen.  Any pointer group may be NULL. */
+struct HtpB200LogitsParams {
+  const int32_t  *history;       /* [n_history] token numbers; a row's tokens so far lie together (prompt, then answer);
+                                    numbers outside 0 .. vocab - 1 count for nothing */
+  const int32_t  *history_start; /* [rows + 1], not decreasing, within 0 .. n_history */
+  const int32_t  *prompt_len;    /* [rows] how many of them are the prompt's; NULL: none */
+  const float    *repetition;    /* [rows] divisor, NULL: 1 */
+  const float    *presence;      /* [rows], NULL: 0 */
+  const float    *frequency;     /* [rows], NULL: 0 */
+  const int32_t  *bias_token;    /* [n_bias]; a token that is named twice gets both, added in their order */
+  const float    *bias_value;    /* [n_bias] */
+  const int32_t  *bias_start;    /* [rows + 1], not decreasing, within 0 .. n_bias */
+  const uint32_t *mask;          /* [n_mask_rows][(vocab + 31) / 32]: bit t % 32 of word t / 32 = token t is allowed */
+  const int32_t  *mask_row;      /* [rows] the row's mask, -1: everything is allowed; NULL: row r has mask r */
+  int32_t         n_history;
+  int32_t         n_bias;
+  int32_t         n_mask_rows;
+};
+/* dst[row][t], from y = src[row][t], c = how often t occurs in the row's answer:
+ *   t in the row's history:  y = y > 0 ? y / repetition : y * repetition
+ *   y -= frequency * c + presence * (c > 0);  y += t's biases;  a token that the mask does not allow: -inf
+ * dst may be src (then only what changes is touched); otherwise they do not overlap.  Rows lie `stride`
+ * elements apart (at least vocab), both pointers 16-byte aligned; what lies between vocab and stride is
+ * left alone. */
+int htp_b200_logits_process(float *dst, const float *src, int64_t stride, int rows, int vocab,
+                            const struct HtpB200LogitsParams *params, void *stream);
+
 /* Waits for `stream`, then returns and clears the first error code a kernel recorded on it
- * (0 = none), or -2 when the stream itself is in error. */
+ * (0 = none), or -2 when the stream itself is in error.  The operators on a paged cache and on logits record
+ * theirs per device, not per stream: 301 a page number out of range, 302 a sequence's row or context
+ * lengths out of range, 303 a position outside the rotation table, 304 history or bias ranges, 305 a mask
+ * row out of range. */
 int htp_b200_stream_status(void *stream);
 
 /* Tuning / debugging switches: "pdl" (programmatic dependent launch, default 1),
