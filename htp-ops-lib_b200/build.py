@@ -14,7 +14,7 @@ LIB = PKG / "libhtp_ops_b200.so"
 
 # Every translation unit of the library.
 SOURCES = ["api.cu", "gemv_mma.cu", "aux_kernels.cu", "host.cu", "no_alloc.cu", "gemm_tcgen05.cu", "tiled_weights.cu",
-           "decoder_ops.cu", "kv_append.cu", "attn_decode.cu", "residual_norm.cu", "logits.cu"]
+           "decoder_ops.cu", "kv_append.cu", "attn_decode.cu", "attn_prompt.cu", "residual_norm.cu", "logits.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,0 +1,57 @@
+// What the two attention kernels over the paged 8-bit cache share: exact conversion of codes, the two-term
+// split of fp32 values, and the constants of the lagging maximum (see attn_decode.cu).
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "decoder_common.cuh"
+#include "unpack.cuh"
+
+namespace htp {
+
+constexpr float kLift  = 8.f;     // weights are kept times 2^8: fp16 terms of small weights stay normal numbers
+constexpr float kSlack = 6.f;     // M may lag the maximum by this much: weights stay below 2^(8 + 6) < 65504
+constexpr float kFloor = -1e30f;  // M before the first score
+
+// Four codes (lowest byte first) as two fp16 pairs.
+template <int KVT>
+__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t (&h)[2]) {
+  if constexpr (KVT == kKvI8) {
+    q8_0_unpack_word(w, h);
+  } else {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w & 0xffff), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w >> 16), __NV_E4M3);
+    h[0]                = (uint32_t) a.x | (uint32_t) a.y << 16;
+    h[1]                = (uint32_t) b.x | (uint32_t) b.y << 16;
+  }
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
+  return h2_as_u32(__floats2half2_rn(a, b));
+}
+
+// hi + lo fp16 terms of two fp32 values
+__device__ __forceinline__ void split_h2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2  f = __half22float2(h);
+  hi              = h2_as_u32(h);
+  lo              = pack_h2(a - f.x, b - f.y);
+}
+
+// The power of two that brings a row's largest magnitude into [2^13, 2^14) - nothing overflows fp16, the
+// second term keeps its bits -, as what to multiply by and what that has to be undone with.
+__device__ __forceinline__ void query_unit(float amax, float &unit, float &by) {
+  int e = ((__float_as_int(amax) >> 23) & 0xff) - 127 - 13;
+  e     = amax == 0.f ? 0 : (e < -100 ? -100 : e);
+  unit  = __int_as_float((127 + e) << 23);
+  by    = __int_as_float((127 - e) << 23);
+}
+
+// The weight of a score.  Scores so large that their rounding exceeds kSlack stay finite; NaN stays NaN.
+__device__ __forceinline__ float weight_of(float y) {
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(kLift + kSlack));
+  return exp2_approx(y);
+}
+
+}  // namespace htp

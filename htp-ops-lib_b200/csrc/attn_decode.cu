@@ -23,9 +23,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include "decoder_common.cuh"
+#include "attn_common.cuh"
 #include "ptx.cuh"
-#include "unpack.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -36,45 +35,10 @@ namespace {
 constexpr int   kWarps   = 4;
 constexpr int   kThreads = kWarps * 32;
 constexpr int   kStep    = 32;     // tokens of a warp's step: two 16-token MMA tiles
-constexpr float kLift    = 8.f;    // weights are kept times 2^8: fp16 terms of small weights stay normal numbers
-constexpr float kSlack   = 6.f;    // M may lag the maximum by this much: weights stay below 2^(8 + 6) < 65504
-constexpr float kFloor   = -1e30f; // M before the first score
-
-// Four codes (lowest byte first) as two fp16 pairs.
-template <int KVT>
-__device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t (&h)[2]) {
-  if constexpr (KVT == kKvI8) {
-    q8_0_unpack_word(w, h);
-  } else {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w & 0xffff), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w >> 16), __NV_E4M3);
-    h[0]                = (uint32_t) a.x | (uint32_t) a.y << 16;
-    h[1]                = (uint32_t) b.x | (uint32_t) b.y << 16;
-  }
-}
-
-__device__ __forceinline__ uint32_t pack_h2(float a, float b) {
-  return h2_as_u32(__floats2half2_rn(a, b));
-}
-
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
-}
-
-// hi + lo fp16 terms of two fp32 values
-__device__ __forceinline__ void split_h2(float a, float b, uint32_t &hi, uint32_t &lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2  f = __half22float2(h);
-  hi              = h2_as_u32(h);
-  lo              = pack_h2(a - f.x, b - f.y);
-}
-
-// The weight of a score.  Scores so large that their rounding exceeds kSlack stay finite; NaN stays NaN.
-__device__ __forceinline__ float weight_of(float y) {
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(kLift + kSlack));
-  return exp2_approx(y);
 }
 
 template <int KVT, int D, int NT, bool F32>
@@ -150,12 +114,11 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       for (int o = D / 8; o > 0; o >>= 1) {  // (the D / 4 lanes of a column: a warp, or half of one)
         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       }
-      int e = ((__float_as_int(m) >> 23) & 0xff) - 127 - 13;
-      e     = m == 0.f ? 0 : (e < -100 ? -100 : e);
-      const float f = __int_as_float((127 - e) << 23);
+      float unit, f;
+      query_unit(m, unit, f);
       v.x *= f, v.y *= f, v.z *= f, v.w *= f;
       if (d == 0) {
-        q_unit[c] = __int_as_float((127 + e) << 23);
+        q_unit[c] = unit;
       }
     }
     uint2 h, l;
@@ -607,17 +570,26 @@ cudaError_t launch_tiles(const AttnArgs &a, const AttnPlan &p, bool pdl, cudaStr
   if (grid > 0x7fffffffll) {
     return cudaErrorInvalidConfiguration;
   }
-  cudaError_t e = p.col_tiles == 1
+  const cudaError_t e = p.col_tiles == 1
                     ? launch_decoder_kernel(attn_decode_kernel<KVT, D, 1, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st)
                     : launch_decoder_kernel(attn_decode_kernel<KVT, D, 2, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st);
-  if (e == cudaSuccess && p.groups > 1) {
-    const long long rows = (long long) a.kv.n_seqs * a.max_q * a.n_heads;
-    e = launch_decoder_kernel(attn_join_kernel<D, F32>, a, (unsigned) ((rows + 3) / 4), 128, 0, pdl, 1, st);
-  }
-  return e;
+  return e != cudaSuccess || p.groups == 1 ? e : attn_join_launch(a, D, !F32, pdl, st);
 }
 
 }  // namespace
+
+cudaError_t attn_join_launch(const AttnArgs &a, int head_dim, bool a16, bool pdl, cudaStream_t st) {
+  const long long rows = (long long) a.kv.n_seqs * a.max_q * a.n_heads, grid = (rows + 3) / 4;
+  if (grid > 0x7fffffffll) {
+    return cudaErrorInvalidConfiguration;
+  }
+  if (head_dim == 64) {
+    return a16 ? launch_decoder_kernel(attn_join_kernel<64, false>, a, (unsigned) grid, 128, 0, pdl, 1, st)
+               : launch_decoder_kernel(attn_join_kernel<64, true>, a, (unsigned) grid, 128, 0, pdl, 1, st);
+  }
+  return a16 ? launch_decoder_kernel(attn_join_kernel<128, false>, a, (unsigned) grid, 128, 0, pdl, 1, st)
+             : launch_decoder_kernel(attn_join_kernel<128, true>, a, (unsigned) grid, 128, 0, pdl, 1, st);
+}
 
 size_t attn_part_bytes(int n_seqs, int max_q, int n_heads, int head_dim, int groups) {
   return groups > 1 ? (size_t) groups * n_seqs * max_q * n_heads * (head_dim + 4) * sizeof(float) : 0;
@@ -627,24 +599,35 @@ AttnPlan attn_plan(int sm_count, int n_seqs, int n_rows, int n_kv_heads, int gro
                    size_t workspace_bytes, int head_dim) {
   AttnPlan        p    = {};
   const long long cols = (long long) max_q * group;
-  p.col_tiles          = cols > 8 ? 2 : 1;
-  p.col_groups         = (int) ((cols + 8 * p.col_tiles - 1) / (8 * p.col_tiles));
-  // enough CTAs for about four on every SM, none with less than a step per warp
-  const long long jobs = (long long) n_seqs * n_kv_heads * p.col_groups, want = 4ll * sm_count;
-  const long long most = ((long long) max_ctx + kStep * kWarps - 1) / (kStep * kWarps);
-  p.splits             = 1;
-  while (p.splits < 8 && jobs * p.splits < want && p.splits < most) {
-    p.splits *= 2;
+  p.splits = p.groups = p.col_tiles = p.col_groups = 1;
+  long long jobs, want, least;  // CTAs of one pass over the contexts, CTAs wanted, tokens worth a CTA of its own
+  if (cols > 32 && group <= 128) {
+    p.tile              = true;
+    const int per_tile  = 128 / group;
+    p.two_row_tiles     = !f32 && max_q > per_tile;
+    const int per_cta   = p.two_row_tiles ? 2 * per_tile : per_tile;
+    p.row_slots         = n_rows / per_cta + (long long) n_seqs;
+    jobs                = ((long long) n_rows + per_cta - 1) / per_cta * n_kv_heads;
+    want = sm_count, least = 1024;
+  } else {
+    p.col_tiles  = cols > 8 ? 2 : 1;
+    p.col_groups = (int) ((cols + 8 * p.col_tiles - 1) / (8 * p.col_tiles));
+    // enough CTAs for about four on every SM, none with less than a step per warp
+    jobs = (long long) n_seqs * n_kv_heads * p.col_groups, want = 4ll * sm_count;
+    const long long most = ((long long) max_ctx + kStep * kWarps - 1) / (kStep * kWarps);
+    while (p.splits < 8 && jobs * p.splits < want && p.splits < most) {
+      p.splits *= 2;
+    }
+    jobs *= p.splits;
+    least = p.splits == 8 ? 4096 : 1 << 30;
   }
-  // several clusters over one context: when each still has a few thousand tokens of its own
-  p.groups = 1;
-  while (p.splits == 8 && p.groups < 16 && jobs * 8 * p.groups < want && (long long) max_ctx / (2 * p.groups) >= 4096) {
+  // several CTAs (clusters) over one context whose results a second launch joins: when each still has enough tokens
+  while (p.groups < 16 && jobs * p.groups < want && max_ctx / (2 * p.groups) >= least) {
     p.groups *= 2;
   }
   while (p.groups > 1 && attn_part_bytes(n_seqs, max_q, n_kv_heads * group, head_dim, p.groups) > workspace_bytes) {
     p.groups /= 2;
   }
-  (void) n_rows, (void) f32;
   return p;
 }
 

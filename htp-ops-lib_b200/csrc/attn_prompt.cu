@@ -1,0 +1,611 @@
+// Attention over the paged 8-bit cache for many rows per sequence (formula: include/htp_ops_b200.h,
+// htp_b200_attn_paged), on the 5th-generation tensor cores.
+//
+// A tile is 128 rows = query rows x heads of one key/value head, against 128 keys at a time:
+//   S = Q . K^T (128 x 128 fp32, tensor memory)      A = Q, B = K in shared memory
+//   O += P . V  (128 x head_dim fp32, tensor memory) A = P in tensor memory, over S; B = V in shared memory
+// Two streams of such tiles run in one CTA, each with its own S, O and four softmax warps, so that one
+// stream's softmax runs under the other's matrix products:
+//   ROWS  two row tiles walk the same keys: the keys' conversion is shared by 256 rows;
+//   KEYS  one row tile, the streams take the key tiles in turn and join their results at the end: fp32
+//         queries, whose two fp16 terms fill the room of the second row tile, and short prompts.
+//
+// Codes become fp16 exactly in four converter warps (global memory -> registers -> 128-byte swizzled shared
+// memory, the next tile's loads in flight meanwhile); scales are applied as in attn_decode.cu: a weight is
+// 2^(s * k_scale * scale * log2 e + log2 v_scale - M), the denominator divides v_scale out again.  fp32 weights are
+// two fp16 terms each.  M follows the row's maximum only when it lags by more than kSlack, so O is rarely rescaled.
+//
+// Bound: per 128 x 128 scores 1024 cycles of tensor core at head_dim 128 and as many of the exponential unit
+// (16 per cycle and SM); fp32 doubles the tensor-core part.
+//
+// Roles: warps 0-3 and 4-7 softmax of stream 0 and 1 (thread = row = TMEM lane), 8-11 converters, 12 MMA
+// issuer and tensor-memory owner.  All waits are bounded; one that runs out records error 311, raises the abort
+// flag, and every role leaves.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "attn_common.cuh"
+#include "ptx.cuh"
+#include "tcgen05.cuh"
+
+namespace htp {
+
+namespace {
+
+constexpr int kSoftWarps = 8;
+constexpr int kConvWarp0 = 8;
+constexpr int kMmaWarp   = 12;
+constexpr int kThreads   = 13 * 32;
+constexpr int kKeys      = 128;  // keys of a tile
+constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more than a softmax warp may lag behind
+
+struct Bars {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
+  uint32_t tmem;
+  int      abort_flag;
+  float    by[kScaleRing][8], up[kScaleRing][8], inv[kScaleRing][8];  // of the tile's 16-key blocks
+  float    unit[128];     // fp32 queries: the power of two that a row was divided by
+  float    ml[2][2][128];  // KEYS: maximum and denominator of each stream's rows
+};
+
+template <int D>
+struct Sizes {
+  static constexpr int kTile = 128 * D * 2;  // 128 rows of fp16
+  // two query parts, two key and two value tiles; at least half of an SM's, so that two CTAs never wait
+  // for each other's tensor memory
+  static constexpr int kSmem = (6 * kTile > 120 * 1024 ? 6 * kTile : 120 * 1024) + 1024 + (int) sizeof(Bars);
+  static_assert(kSmem <= 232448, "shared memory");
+};
+
+struct Waiter {
+  volatile int *abort_flag;
+  int          *err;
+  // the whole warp waits; true when the barrier's phase has completed
+  __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity) const {
+    bool ok = false;
+    for (uint32_t i = 0; i < kWaitCap && !ok; ++i) {
+      ok = mbar_try_wait(bar, parity);
+      if (!ok && i >= 4096) {
+        if (*abort_flag) {
+          break;
+        }
+        __nanosleep(128);
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && *abort_flag == 0) {
+      record_error(err, kErrWait);
+      *abort_flag = 1;
+    }
+    return ok;
+  }
+};
+
+// byte offset of the 16-byte chunk `c` (8 halves) of row `r` in a 128-row operand tile: 64 halves of all rows
+// after each other, 128-byte swizzle
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t) ((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+template <int KVT, int D, bool F32, bool ROWS>
+__global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_constant__ AttnArgs a) {
+  static_assert(!(F32 && ROWS), "fp32 queries take the room of both row tiles");
+  constexpr int TILE  = Sizes<D>::kTile;
+  constexpr int TERMS = F32 ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t) 1023);
+  uint8_t *sQ = smem, *sK = smem + 2 * TILE, *sV = smem + 4 * TILE;
+  Bars    *bar = reinterpret_cast<Bars *>(smem + 6 * TILE);
+  pdl_launch_dependents();
+  pdl_wait_prior_grids();
+
+  const KvView &kv   = a.kv;
+  const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // ---- which rows: sequence b has the row blocks from q_start[b] / per_cta + b on, at least as many as it
+  // needs; late blocks first, they see the most keys
+  const int per_tile = 128 / a.group;  // query rows of a tile
+  const int per_cta  = ROWS ? 2 * per_tile : per_tile;
+  unsigned  id       = blockIdx.x;
+  const int grp      = id % a.groups;
+  id /= a.groups;
+  const int head = id % kv.n_kv_heads;
+  id /= kv.n_kv_heads;
+  const long long slot = (long long) (a.row_slots - 1) - id;
+  auto            at   = [&](int i) { return (long long) (kv.q_start[i] / per_cta) + i; };
+  const int       b    = interval_of(kv.n_seqs, slot, at);
+  if (b >= kv.n_seqs) {
+    return;
+  }
+  int q0, q_len, ctx;
+  if (!sequence_of(kv, b, a.max_q, a.max_ctx, q0, q_len, ctx)) {
+    if (threadIdx.x == 0) {
+      record_error(a.err, kErrSequence);
+    }
+    return;
+  }
+  const long long block = slot - at(b);
+  if (block < 0 || block * per_cta >= q_len) {
+    return;
+  }
+  const int i0 = (int) block * per_cta, i1 = i0 + per_cta < q_len ? i0 + per_cta : q_len;
+  const int past = ctx - q_len;
+  int       lo = 0, hi = past + i1;
+  hi = hi < 0 ? 0 : hi;
+  if (a.window > 0 && past + i0 - a.window + 1 > 0) {
+    lo = past + i0 - a.window + 1;
+  }
+  int       first_tile = lo / kKeys, n = hi > lo ? (hi + kKeys - 1) / kKeys - first_tile : 0;
+  const int share0 = (int) ((long long) n * grp / a.groups), share1 = (int) ((long long) n * (grp + 1) / a.groups);
+  first_tile += share0;
+  n = share1 - share0;  // key tiles of this CTA
+  // tile j of stream x is key tile j (ROWS) or 2 j + x (KEYS)
+  const int n_of[2] = { ROWS ? n : (n + 1) / 2, ROWS ? n : n / 2 };
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar->q_full, kSoftWarps);
+    mbar_init(&bar->drained, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->k_full[i], 4), mbar_init(&bar->k_empty[i], 1);
+      mbar_init(&bar->v_full[i], 4), mbar_init(&bar->v_empty[i], 1);
+      mbar_init(&bar->s_full[i], 2), mbar_init(&bar->p_ready[i], 4), mbar_init(&bar->o_done[i], 1);
+    }
+    bar->abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc<false>(&bar->tmem, 512);
+    tmem_relinquish<false>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&bar->tmem);
+  const Waiter   wait{ &bar->abort_flag, a.err };
+  auto           s_at = [&](int x) { return tmem + (uint32_t) x * 128; };
+  auto           o_at = [&](int x) { return tmem + 256 + (uint32_t) x * 128; };
+
+  if (warp < kSoftWarps) {
+    // ---------------- softmax
+    const int x = warp >> 2, row = (warp & 3) * 32 + lane;
+    // queries -> shared memory: 128 rows of `parts` tiles
+    constexpr int CH = D / 8;  // 16-byte chunks of a row
+    for (int i = threadIdx.x; i < (ROWS ? 2 : 1) * 128 * CH; i += kSoftWarps * 32) {
+      const int part = i / (128 * CH), r = i / CH % 128, c = i % CH;
+      const int q    = i0 + part * per_tile + r / a.group;
+      const bool in  = r < per_tile * a.group && q < i1;
+      const long long at_q = (long long) (q0 + q) * a.q_stride + (head * a.group + r % a.group) * D + c * 8;
+      uint8_t        *to   = sQ + part * TILE + chunk_at(r, c);
+      if constexpr (F32) {
+        float v[8] = {};
+        if (in) {
+          const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at_q);
+          const float4 w = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at_q + 4);
+          v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
+        }
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          m = fmaxf(m, fabsf(v[e]));
+        }
+#pragma unroll
+        for (int o = CH / 2; o > 0; o >>= 1) {  // (CH lanes hold a row)
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        float unit, by;
+        query_unit(m, unit, by);
+        if (c == 0) {
+          bar->unit[r] = unit;
+        }
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          split_h2(v[2 * e] * by, v[2 * e + 1] * by, h[e], l[e]);
+        }
+        *reinterpret_cast<uint4 *>(to)        = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+      } else {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (in) {
+          v = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at_q);
+        }
+        *reinterpret_cast<uint4 *>(to) = v;
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(&bar->q_full);
+    }
+    bool ok = wait(&bar->q_full, 0);  // (the rows' units)
+    const float unit = F32 ? bar->unit[row] : 1.f;
+
+    const int  my_q   = i0 + (ROWS ? x * per_tile : 0) + row / a.group;
+    const bool mine   = row < per_tile * a.group && my_q < i1;
+    // rows that are nobody's see everything: they cost no mask, and are not stored
+    const int last  = mine ? past + my_q : 0x7fffffff;
+    const int first = mine && a.window > 0 ? past + my_q - a.window + 1 : (int) 0x80000000;
+    const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16;
+    const uint32_t s_addr = s_at(x) + lanes, o_addr = o_at(x) + lanes;
+    float          mx = kFloor, l = 0.f;
+    for (int j = 0; j < n_of[x] && ok; ++j) {
+      const int    t    = ROWS ? j : 2 * j + x;
+      const int    key0 = (first_tile + t) * kKeys;
+      const float *by_ = bar->by[t % kScaleRing], *up_ = bar->up[t % kScaleRing], *inv_ = bar->inv[t % kScaleRing];
+      if (!(ok = wait(&bar->s_full[x], j & 1))) {
+        break;
+      }
+      tc_fence_after();
+      const bool full = __all_sync(0xffffffffu, key0 >= first && key0 + kKeys - 1 <= last);
+      // ---- the row's largest score of this tile
+      float top = kFloor;
+      uint32_t s[32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld32_issue(s_addr + 32 * c, s);
+        tmem_ld_wait32(s);
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int key = key0 + 32 * c + e;
+            s[e] = key <= last && key >= first ? s[e] : 0xff800000u;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float m = __uint_as_float(s[16 * h]);
+#pragma unroll
+          for (int e = 1; e < 16; ++e) {
+            m = fmaxf(m, __uint_as_float(s[16 * h + e]));
+          }
+          top = fmaxf(top, fmaf(m, by_[2 * c + h] * unit, up_[2 * c + h]));
+        }
+      }
+      if (__any_sync(0xffffffffu, top > mx + kSlack)) {
+        const float m = fmaxf(mx, top), f = exp2_approx(mx - m);
+        mx = m;
+        l *= f;
+        if (j > 0) {
+          if (!(ok = wait(&bar->o_done[x], (j - 1) & 1))) {
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            tmem_ld32_issue(o_addr + 32 * c, s);
+            tmem_ld_wait32(s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
+            }
+            tmem_st32(o_addr + 32 * c, s);
+          }
+        }
+      }
+      // ---- weights, over the scores: 32 keys in the first 16 of their 32 columns, second terms in the others
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld32_issue(s_addr + 32 * c, s);
+        tmem_ld_wait32(s);
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int key = key0 + 32 * c + e;
+            s[e] = key <= last && key >= first ? s[e] : 0xff800000u;
+          }
+        }
+        uint32_t p[16], p2[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float by = by_[2 * c + h] * unit, up = up_[2 * c + h] - mx + kLift;
+          float       sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const float u = weight_of(fmaf(__uint_as_float(s[16 * h + e]), by, up));
+            const float v = weight_of(fmaf(__uint_as_float(s[16 * h + e + 1]), by, up));
+            sum += u;
+            sum += v;
+            if constexpr (F32) {
+              split_h2(u, v, p[8 * h + e / 2], p2[8 * h + e / 2]);
+            } else {
+              p[8 * h + e / 2] = pack_h2(u, v);
+            }
+          }
+          l = fmaf(sum, inv_[2 * c + h], l);
+        }
+        tmem_st16(s_addr + 32 * c, p);
+        if constexpr (F32) {
+          tmem_st16(s_addr + 32 * c + 16, p2);
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar->p_ready[x]);
+      }
+    }
+    // ---- results
+    if (ok && n_of[x] > 0) {
+      ok = wait(&bar->o_done[x], (n_of[x] - 1) & 1);
+    }
+    float f0 = 1.f, f1 = 0.f;
+    if constexpr (!ROWS) {
+      if (ok && n_of[x ^ 1] > 0) {
+        ok = wait(&bar->o_done[x ^ 1], (n_of[x ^ 1] - 1) & 1);
+      }
+      bar->ml[x][0][row] = mx, bar->ml[x][1][row] = l;
+      named_bar_sync(1, kSoftWarps * 32);
+      const float m = fmaxf(bar->ml[0][0][row], bar->ml[1][0][row]);
+      f0 = exp2_approx(bar->ml[0][0][row] - m), f1 = exp2_approx(bar->ml[1][0][row] - m);
+      l  = fmaf(f1, bar->ml[1][1][row], f0 * bar->ml[0][1][row]);
+      mx = m;
+    }
+    tc_fence_after();
+    if (ok) {
+      const int  h  = head * a.group + row % a.group;
+      const bool part = a.groups > 1;
+      const float scale = part ? 1.f : (l > 0.f ? 1.f / l : 0.f);
+      float      *to = part ? a.part + ((((long long) grp * kv.n_seqs + b) * a.max_q + my_q) * a.n_heads + h) * (D + 4) : nullptr;
+      const long long at_o = (long long) (q0 + my_q) * a.out_stride + h * D;
+      if (part && mine && (ROWS || x == 0)) {
+        *reinterpret_cast<float2 *>(to + D) = make_float2(mx, l);
+      }
+      __syncwarp();
+      // ROWS: every thread stores its row; KEYS: the streams' warps store one half of the columns each
+      constexpr int C0 = ROWS ? D / 32 : D / 64;
+#pragma unroll
+      for (int k = 0; k < C0; ++k) {
+        const int c = ROWS ? k : x * C0 + k;
+        float     v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          v[e] = 0.f;
+        }
+#pragma unroll
+        for (int y = 0; y < (ROWS ? 1 : 2); ++y) {
+          const int   z = ROWS ? x : y;
+          const float f = (y ? f1 : f0) * scale;
+          if (n_of[z] > 0) {
+            uint32_t o[32];
+            tmem_ld32_issue(o_at(z) + lanes + 32 * c, o);
+            tmem_ld_wait32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              v[e] = fmaf(__uint_as_float(o[e]), f, v[e]);
+            }
+          }
+        }
+        if (!mine) {
+        } else if (part || F32) {
+          float *dst = part ? to + 32 * c : static_cast<float *>(a.out) + at_o + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            *reinterpret_cast<float4 *>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          }
+        } else {
+          __half *dst = static_cast<__half *>(a.out) + at_o + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            *reinterpret_cast<uint4 *>(dst + e) = make_uint4(pack_h2(v[e], v[e + 1]), pack_h2(v[e + 2], v[e + 3]),
+                                                             pack_h2(v[e + 4], v[e + 5]), pack_h2(v[e + 6], v[e + 7]));
+          }
+        }
+        __syncwarp();  // (the next tensor-memory load is the whole warp's)
+      }
+    }
+    tc_fence_before();
+  } else if (warp < kMmaWarp) {
+    // ---------------- converters: a warp takes 32 keys (two 16-key blocks) of every tile
+    constexpr int PIECES = D / 16;            // 16-byte pieces of a key's codes
+    constexpr int RPL    = 32 / PIECES;       // keys of one warp-wide load
+    constexpr int LOADS  = 32 / RPL;          // loads of a lane per tile
+    const int cw = warp - kConvWarp0, piece = lane % PIECES, sub = lane / PIECES;
+    const int     *table = kv.page_table + (long long) b * kv.table_stride;
+    // page of block i (0, 1) of this warp's keys in tile t; -1: nothing there, -2: a bad entry
+    auto page_of = [&](int t, int i) {
+      const int key = (first_tile + t) * kKeys + cw * 32 + 16 * i;
+      if (t >= n || key >= hi || key + 16 <= lo) {
+        return -1;
+      }
+      const int p = table[key >> kv.page_shift];
+      if (p < 0 || p >= kv.n_pages) {
+        if (lane == 0) {
+          record_error(a.err, kErrPage);
+        }
+        return -2;
+      }
+      return p;
+    };
+    auto load = [&](const uint8_t *codes, int t, const int (&pg)[2], uint4 (&r)[LOADS]) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int k = i * RPL + sub, key = (first_tile + t) * kKeys + cw * 32 + k, p = pg[i >= LOADS / 2];
+        r[i] = make_uint4(0, 0, 0, 0);  // (zeros behind the context: what lies there may be no numbers)
+        if (p >= 0 && key < hi && key >= lo) {
+          r[i] = ld_stream16(codes + ((((long long) p * kv.n_kv_heads + head) << kv.page_shift) + (key & (kv.page_size - 1))) * D + piece * 16);
+        }
+      }
+    };
+    auto convert = [&](uint8_t *tile, const uint4 (&r)[LOADS]) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int      k = cw * 32 + i * RPL + sub;
+        const uint32_t w[4] = { r[i].x, r[i].y, r[i].z, r[i].w };
+        uint32_t       h[4][2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          codes_to_h2<KVT>(w[e], h[e]);
+        }
+        const uint4 c0 = make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]), c1 = make_uint4(h[2][0], h[2][1], h[3][0], h[3][1]);
+        // (the upper half of a key's pieces stores its chunks in the other order: no two lanes of a row on one bank)
+        const int swap = D == 128 ? piece >> 2 : 0;
+        *reinterpret_cast<uint4 *>(tile + chunk_at(k, 2 * piece + swap))     = swap ? c1 : c0;
+        *reinterpret_cast<uint4 *>(tile + chunk_at(k, 2 * piece + 1 - swap)) = swap ? c0 : c1;
+      }
+    };
+    auto publish = [&](uint64_t *full) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(full);
+      }
+    };
+    uint4 rk[LOADS], rv[LOADS];
+    int   pg[2] = { page_of(0, 0), page_of(0, 1) }, pn[2];
+    load(kv.k_codes, 0, pg, rk);
+    bool ok = true;
+    for (int t = 0; t < n && ok; ++t) {
+      const int      i = t & 1;
+      const uint32_t parity = ((t >> 1) & 1) ^ 1;
+      load(kv.v_codes, t, pg, rv);
+      float by = a.scale_log2, up = -INFINITY, inv = 0.f;
+      const int p = lane == 0 ? pg[0] : pg[1];
+      if (lane < 2 && p >= 0) {
+        const float ks = kv.k_scale[(long long) p * kv.n_kv_heads + head], vs = kv.v_scale[(long long) p * kv.n_kv_heads + head];
+        const float v = vs > 0.f ? vs : 1.f;
+        by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = log2f(v), inv = 1.f / v;
+      }
+      pn[0] = page_of(t + 1, 0), pn[1] = page_of(t + 1, 1);
+      if (!(ok = wait(&bar->k_empty[i], parity))) {
+        break;
+      }
+      if (lane < 2) {
+        bar->by[t % kScaleRing][2 * cw + lane] = by, bar->up[t % kScaleRing][2 * cw + lane] = up;
+        bar->inv[t % kScaleRing][2 * cw + lane] = inv;
+      }
+      convert(sK + i * TILE, rk);
+      publish(&bar->k_full[i]);
+      if (t + 1 < n) {
+        load(kv.k_codes, t + 1, pn, rk);
+      }
+      if (!(ok = wait(&bar->v_empty[i], parity))) {
+        break;
+      }
+      convert(sV + i * TILE, rv);
+      publish(&bar->v_full[i]);
+      pg[0] = pn[0], pg[1] = pn[1];
+    }
+  } else {
+    // ---------------- MMA issuer: the whole warp walks the loop, one elected lane issues
+    constexpr uint32_t IDESC_S = instr_desc_f16(128, kKeys), IDESC_O = instr_desc_f16(128, D) | kInstrBMajorMn;
+    bool ok = n == 0 || wait(&bar->q_full, 0);
+    auto scores = [&](int x, int j) {
+      const int t = ROWS ? j : 2 * j + x, i = t & 1;
+      if (!ROWS || x == 0) {
+        ok = ok && wait(&bar->k_full[i], (t >> 1) & 1);
+      }
+      if (!ok) {
+        return;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t kd = smem_desc_sw128(sK + i * TILE);
+#pragma unroll
+        for (int term = 0; term < TERMS; ++term) {
+          const uint64_t qd = smem_desc_sw128(sQ + (ROWS ? x : term) * TILE);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+            umma_f16_ss(s_at(x), qd + off, kd + off, IDESC_S, (term | k) ? 1u : 0u);
+          }
+        }
+        umma_commit<false>(&bar->s_full[x]);
+        mbar_arrive(&bar->s_full[x]);  // (carries the converters' scales on to the softmax warps)
+        if (!ROWS || x == 1) {
+          umma_commit<false>(&bar->k_empty[i]);
+        }
+      }
+      __syncwarp();
+    };
+    for (int x = 0; x < 2 && ok; ++x) {
+      if (n_of[x] > 0) {
+        scores(x, 0);
+      }
+    }
+    for (int j = 0; j < n_of[0] && ok; ++j) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (j >= n_of[x] || !ok) {
+          continue;
+        }
+        const int t = ROWS ? j : 2 * j + x, i = t & 1;
+        if (!ROWS || x == 0) {
+          ok = wait(&bar->v_full[i], (t >> 1) & 1);
+        }
+        ok = ok && wait(&bar->p_ready[x], j & 1);
+        if (!ok) {
+          continue;
+        }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = smem_desc_sw128_mn(sV + i * TILE, 16384);
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k) {
+#pragma unroll
+            for (int term = 0; term < TERMS; ++term) {
+              umma_f16_ts<false>(o_at(x), s_at(x) + 32 * (k >> 1) + 8 * (k & 1) + 16 * term, vd + k * (2048 >> 4), IDESC_O,
+                                 (j | k | term) ? 1u : 0u);
+            }
+          }
+          umma_commit<false>(&bar->o_done[x]);
+          if (!ROWS || x == 1) {
+            umma_commit<false>(&bar->v_empty[i]);
+          }
+        }
+        __syncwarp();
+        if (j + 1 < n_of[x]) {
+          scores(x, j + 1);
+        }
+      }
+    }
+    if (!ok) {  // what has been issued still reads shared memory: let it end
+      if (elect_one()) {
+        umma_commit<false>(&bar->drained);
+      }
+      __syncwarp();
+      for (uint32_t i = 0; i < kWaitCap && !mbar_try_wait(&bar->drained, 0); ++i) {
+        __nanosleep(64);
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<false>(tmem, 512);
+  }
+}
+
+template <int KVT, int D, bool F32, bool ROWS>
+cudaError_t launch(const AttnArgs &a, bool pdl, cudaStream_t st) {
+  const long long grid = a.row_slots * a.kv.n_kv_heads * a.groups;
+  if (grid > 0x7fffffffll) {
+    return cudaErrorInvalidConfiguration;
+  }
+  constexpr int     smem = Sizes<D>::kSmem;
+  const cudaError_t e    = cudaFuncSetAttribute(attn_prompt_kernel<KVT, D, F32, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  return e != cudaSuccess ? e : launch_decoder_kernel(attn_prompt_kernel<KVT, D, F32, ROWS>, a, (unsigned) grid, kThreads, smem, pdl, 1, st);
+}
+
+template <int KVT, int D>
+cudaError_t launch_type(const AttnArgs &a, const AttnPlan &p, bool a16, bool pdl, cudaStream_t st) {
+  if (!a16) {
+    return launch<KVT, D, true, false>(a, pdl, st);
+  }
+  return p.two_row_tiles ? launch<KVT, D, false, true>(a, pdl, st) : launch<KVT, D, false, false>(a, pdl, st);
+}
+
+}  // namespace
+
+cudaError_t attn_prompt_launch(const AttnArgs &a, const AttnPlan &p, int head_dim, int kv_type, bool a16, bool pdl,
+                               cudaStream_t st) {
+  cudaError_t e;
+  if (head_dim == 64) {
+    e = kv_type == kKvI8 ? launch_type<kKvI8, 64>(a, p, a16, pdl, st) : launch_type<kKvE4m3, 64>(a, p, a16, pdl, st);
+  } else {
+    e = kv_type == kKvI8 ? launch_type<kKvI8, 128>(a, p, a16, pdl, st) : launch_type<kKvE4m3, 128>(a, p, a16, pdl, st);
+  }
+  return e != cudaSuccess || p.groups == 1 ? e : attn_join_launch(a, head_dim, a16, pdl, st);
+}
+
+}  // namespace htp

@@ -219,9 +219,10 @@ int htp_b200_attn_paged(void *out, int64_t out_stride, const void *q, int64_t q_
   a.n_heads    = n_heads;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.window = window, a.max_q = max_q, a.max_ctx = max_ctx;
-  a.col_groups = p.col_groups, a.splits = p.splits, a.groups = p.groups;
-  return done(attn_decode_launch(a, p, kv->head_dim, kv->kv_type, act_type == HTP_B200_ACT_F16, g_opt_pdl != 0,
-                                 static_cast<cudaStream_t>(stream)),
+  a.col_groups = p.col_groups, a.splits = p.splits, a.groups = p.groups, a.row_slots = p.row_slots;
+  const auto launch = p.tile ? attn_prompt_launch : attn_decode_launch;
+  return done(launch(a, p, kv->head_dim, kv->kv_type, act_type == HTP_B200_ACT_F16, g_opt_pdl != 0,
+                     static_cast<cudaStream_t>(stream)),
               p.groups > 1 ? 2 : 1);
 }
 

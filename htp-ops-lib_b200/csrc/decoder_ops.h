@@ -13,6 +13,7 @@ constexpr int kErrSequence = 302;
 constexpr int kErrPosition = 303;
 constexpr int kErrRange    = 304;
 constexpr int kErrMaskRow  = 305;
+constexpr int kErrWait     = 311;  // a bounded wait inside the prompt attention ran out
 
 constexpr float kKvMinScale = 0x1p-100f;  // scale of a block of zeros
 
@@ -46,21 +47,29 @@ struct AttnArgs {
   int         n_heads, group;  // group = query heads of one key/value head
   float       scale_log2;      // scale * log2(e)
   int         window, max_q, max_ctx;
-  int         col_groups, splits, groups;  // splits = CTAs of a cluster, groups = clusters over one context
+  int         col_groups, splits, groups;  // splits = CTAs of a cluster, groups = clusters (CTAs) over one context
+  long long   row_slots;       // attn_prompt.cu: blocks of rows of the grid
   int        *err;
 };
 // How a step is cut: columns of query rows x heads of a key/value head per CTA, CTAs of a cluster and
 // clusters over one context.
 struct AttnPlan {
-  bool tile;        // the kernel for many rows (attn_prompt.cu)
-  int  col_tiles;   // 8-column tiles per CTA
-  int  col_groups, splits, groups;
+  bool      tile;           // the kernel for many rows (attn_prompt.cu)
+  bool      two_row_tiles;  // of it: two tiles of rows per CTA
+  long long row_slots;      // of it: blocks of rows, bounded by what n_rows and n_seqs allow
+  int       col_tiles;      // 8-column tiles per CTA
+  int       col_groups, splits, groups;
 };
 AttnPlan    attn_plan(int sm_count, int n_seqs, int n_rows, int n_kv_heads, int group, bool f32, int max_q, int max_ctx,
                       size_t workspace_bytes, int head_dim);
 size_t      attn_part_bytes(int n_seqs, int max_q, int n_heads, int head_dim, int groups);
 cudaError_t attn_decode_launch(const AttnArgs &a, const AttnPlan &p, int head_dim, int kv_type, bool a16, bool pdl,
                                cudaStream_t stream);
+
+cudaError_t attn_prompt_launch(const AttnArgs &a, const AttnPlan &p, int head_dim, int kv_type, bool a16, bool pdl,
+                               cudaStream_t stream);
+// joins the results of the groups (attn_decode.cu)
+cudaError_t attn_join_launch(const AttnArgs &a, int head_dim, bool a16, bool pdl, cudaStream_t stream);
 
 struct AddRmsNormArgs {
   float       *h_out;

@@ -81,8 +81,10 @@ __device__ __forceinline__ uint32_t to_codes4(const float *x, float by) {
     }
     return w;
   } else {
-    const float2 a = make_float2(__fmul_rn(x[0], by), __fmul_rn(x[1], by));
-    const float2 b = make_float2(__fmul_rn(x[2], by), __fmul_rn(x[3], by));
+    // (NaN: 0, as in signed bytes - a code that is no number would reach rows that do not see its token)
+    auto         c = [&](float v) { return v == v ? __fmul_rn(v, by) : 0.f; };
+    const float2 a = make_float2(c(x[0]), c(x[1]));
+    const float2 b = make_float2(c(x[2]), c(x[3]));
     return (uint32_t) __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
            (uint32_t) __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
   }

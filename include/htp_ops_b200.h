@@ -199,7 +199,8 @@ int htp_b200_rms_norm_f32(float *dst, const float *src, int ne0, int ne1, void *
  * that a code stands for is code * scale.  Sequence b owns rows q_start[b] .. q_start[b + 1] - 1 of the
  * step's row-major inputs; they are the last tokens of its ctx_len[b] (these rows among them), and token j
  * lies in page page_table[b][j / page_size].  Rows from q_start[n_seqs] on belong to nobody: they are
- * neither read nor written.  Entries of the table behind a sequence's last page are not read.  Scales are
+ * neither read nor written.  Entries of the table behind a sequence's last page are not read.  e4m3's codes
+ * that are no number (0x7f, 0xff) do not stand for tokens of a sequence; behind its end any byte may lie.  Scales are
  * positive (0 is taken as 1, for blocks whose codes are all 0); the scales of the value pages one row
  * attends to lie within a factor of 2^110 of each other. */
 struct HtpB200PagedKv {
@@ -242,7 +243,7 @@ struct HtpB200Rope {
  *   needed = max(amax / 127 (signed bytes) or amax / 448 (e4m3), 2^-100),
  *   scale  = needed when the page holds no older tokens of the sequence, else max(its scale, needed);
  * codes of older tokens follow a grown scale: c becomes round(c * (old scale / scale)); new codes are
- * round(x * (1 / scale)), ties to even, saturated (NaN: 0 in signed bytes, NaN in e4m3).  Every step is a
+ * round(x * (1 / scale)), ties to even, saturated (NaN: 0).  Every step is a
  * correctly rounded fp32 operation (products and sums not contracted), so the bytes are reproducible.
  * Appending the same rows twice gives the same cache as once.  A page that is appended to belongs to one
  * sequence, once: two that share it may only read it. */
@@ -314,7 +315,7 @@ int htp_b200_logits_process(float *dst, const float *src, int64_t stride, int ro
  * (0 = none), or -2 when the stream itself is in error.  The operators on a paged cache and on logits record
  * theirs per device, not per stream: 301 a page number out of range, 302 a sequence's row or context
  * lengths out of range, 303 a position outside the rotation table, 304 history or bias ranges, 305 a mask
- * row out of range. */
+ * row out of range; 311 a bounded wait inside the prompt attention ran out. */
 int htp_b200_stream_status(void *stream);
 
 /* Tuning / debugging switches: "pdl" (programmatic dependent launch, default 1),

@@ -16,11 +16,11 @@ def decode(codes, kv, dtype=torch.float64):
 
 
 def encode32(x, kv):
-    """fp32 values as codes: ties to even, saturated; NaN: 0 in signed bytes, NaN in e4m3."""
+    """fp32 values as codes: ties to even, saturated; NaN: 0."""
+    x = torch.nan_to_num(x, nan=0.0, posinf=1e6, neginf=-1e6)
     if kv == "i8":
-        return torch.nan_to_num(torch.round(x), nan=0.0, posinf=127, neginf=-127).clamp(-127, 127).to(torch.int8).view(torch.uint8)
-    y = torch.where(torch.isnan(x), x, x.clamp(-448, 448))
-    return y.to(torch.float8_e4m3fn).view(torch.uint8)
+        return torch.round(x).clamp(-127, 127).to(torch.int8).view(torch.uint8)
+    return x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
 
 
 class Cache:

@@ -22,6 +22,11 @@ SHAPES = [
     ([(1, 20011)], 3, 1, 64, 16),
     ([(40, 77), (7, 7), (1, 300)], 7, 1, 64, 32),
     ([(130, 515), (64, 64)], 8, 2, 128, 64),
+    ([(300, 300), (1, 50), (0, 3), (70, 1200), (129, 100)], 12, 4, 128, 16),  # the last: more rows than tokens
+    ([(33, 3001)], 8, 1, 64, 128),
+    ([(9, 5000), (16, 20)], 16, 2, 128, 32),
+    ([(257, 257)], 5, 5, 64, 64),
+    ([(3, 40), (2, 500)], 130, 1, 64, 16),
 ]
 
 
