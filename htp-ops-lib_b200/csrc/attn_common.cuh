@@ -13,6 +13,10 @@ namespace htp {
 constexpr float kLift  = 8.f;     // weights are kept times 2^8: fp16 terms of small weights stay normal numbers
 constexpr float kSlack = 6.f;     // M may lag the maximum by this much: weights stay below 2^(8 + 6) < 65504
 constexpr float kFloor = -1e30f;  // M before the first score
+// From this M on, folding M into the product's addend (one rounding of numbers as large as M, another one for each
+// block of tokens) would shift the blocks against each other by parts of a power of two: the difference to M
+// is then taken from the rounded score instead, exactly.
+constexpr float kHuge = 65536.f;
 
 // Four codes (lowest byte first) as two fp16 pairs.
 template <int KVT>
@@ -48,10 +52,29 @@ __device__ __forceinline__ void query_unit(float amax, float &unit, float &by) {
   by    = __int_as_float((127 - e) << 23);
 }
 
-// The weight of a score.  Scores so large that their rounding exceeds kSlack stay finite; NaN stays NaN.
-__device__ __forceinline__ float weight_of(float y) {
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(kLift + kSlack));
-  return exp2_approx(y);
+// Two fp32 operations of one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 }  // namespace htp

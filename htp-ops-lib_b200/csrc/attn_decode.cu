@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
     }
   }
-  int pg[2], pn[2];
+  bool huge = false;
+  int  pg[2], pn[2];
   int step = begin + warp;
   pg[0] = page_of(step, 0), pg[1] = page_of(step, 1);
   load_k(step, pg);
@@ -299,6 +300,10 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
         }
       }
     }
+    auto exponent = [&](int m, int n, int e) {
+      const float b = by[m] * unit[n][e & 1], x = mx[n][e & 1];
+      return huge ? fmaf(s[m][n][e], b, up[m]) - x + kLift : fmaf(s[m][n][e], b, up[m] - x + kLift);
+    };
     float y[2][NT][4];
     float top = -INFINITY;
 #pragma unroll
@@ -307,12 +312,13 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[m][n][e] = fmaf(s[m][n][e], by[m] * unit[n][e & 1], up[m] - mx[n][e & 1] + kLift);
+          y[m][n][e] = exponent(m, n, e);
           top        = fmaxf(top, y[m][n][e]);
         }
       }
     }
     if (__any_sync(0xffffffffu, top > kLift + kSlack)) {
+      bool far = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -335,11 +341,16 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
             o[n][i][j + 2] *= f;
           }
         }
+        far = far || (fabsf(mx[n][0]) > kHuge && mx[n][0] != kFloor) || (fabsf(mx[n][1]) > kHuge && mx[n][1] != kFloor);
+      }
+      huge = __any_sync(0xffffffffu, far);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            y[m][n][e] = fmaf(s[m][n][e], by[m] * unit[n][e & 1], up[m] - mx[n][e & 1] + kLift);
+            y[m][n][e] = exponent(m, n, e);
           }
         }
       }
@@ -351,7 +362,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          y[m][n][e] = weight_of(y[m][n][e]);
+          y[m][n][e] = exp2_approx(y[m][n][e]);
         }
         l[n][0] = fmaf(y[m][n][0] + y[m][n][2], inv[m], l[n][0]);
         l[n][1] = fmaf(y[m][n][1] + y[m][n][3], inv[m], l[n][1]);

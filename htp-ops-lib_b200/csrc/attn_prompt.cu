@@ -27,6 +27,7 @@
 #include "attn_common.cuh"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
+#include "unpack.cuh"
 
 namespace htp {
 
@@ -35,7 +36,7 @@ namespace {
 constexpr int kSoftWarps = 8;
 constexpr int kConvWarp0 = 8;
 constexpr int kMmaWarp   = 12;
-constexpr int kThreads   = 13 * 32;
+constexpr int kThreads   = 16 * 32;  // warps 13-15 only lend their registers
 constexpr int kKeys      = 128;  // keys of a tile
 constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more than a softmax warp may lag behind
 
@@ -168,48 +169,60 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
   if (warp < kSoftWarps) {
     // ---------------- softmax
     const int x = warp >> 2, row = (warp & 3) * 32 + lane;
-    // queries -> shared memory: 128 rows of `parts` tiles
-    constexpr int CH = D / 8;  // 16-byte chunks of a row
-    for (int i = threadIdx.x; i < (ROWS ? 2 : 1) * 128 * CH; i += kSoftWarps * 32) {
-      const int part = i / (128 * CH), r = i / CH % 128, c = i % CH;
-      const int q    = i0 + part * per_tile + r / a.group;
-      const bool in  = r < per_tile * a.group && q < i1;
-      const long long at_q = (long long) (q0 + q) * a.q_stride + (head * a.group + r % a.group) * D + c * 8;
-      uint8_t        *to   = sQ + part * TILE + chunk_at(r, c);
-      if constexpr (F32) {
-        float v[8] = {};
-        if (in) {
-          const float4 u = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at_q);
-          const float4 w = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at_q + 4);
-          v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w, v[4] = w.x, v[5] = w.y, v[6] = w.z, v[7] = w.w;
-        }
-        float m = 0.f;
+    // queries -> shared memory: 128 rows of one or two parts, a batch of loads in flight
+    constexpr int CH    = D / 8;  // 16-byte chunks of a row
+    constexpr int ITEMS = (ROWS ? 2 : 1) * 128 * CH / (kSoftWarps * 32), BATCH = F32 ? 4 : 8;
+    static_assert(ITEMS % 4 == 0, "whole batches");
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          m = fmaxf(m, fabsf(v[e]));
-        }
+    for (int i0_ = 0; i0_ < ITEMS; i0_ += BATCH < ITEMS ? BATCH : ITEMS) {
+      constexpr int NB = BATCH < ITEMS ? BATCH : ITEMS;
+      uint4         v[NB][F32 ? 2 : 1];
 #pragma unroll
-        for (int o = CH / 2; o > 0; o >>= 1) {  // (CH lanes hold a row)
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        }
-        float unit, by;
-        query_unit(m, unit, by);
-        if (c == 0) {
-          bar->unit[r] = unit;
-        }
-        uint32_t h[4], l[4];
+      for (int i = 0; i < NB; ++i) {
+        const int  it = threadIdx.x + (i0_ + i) * kSoftWarps * 32, part = it / (128 * CH), r = it / CH % 128, c = it % CH;
+        const int  q  = i0 + part * per_tile + r / a.group;
+        const bool in = r < per_tile * a.group && q < i1;
+        const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.q) +
+                            ((long long) (q0 + q) * a.q_stride + (head * a.group + r % a.group) * D + c * 8) * (F32 ? 4 : 2));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          split_h2(v[2 * e] * by, v[2 * e + 1] * by, h[e], l[e]);
+        for (int u = 0; u < (F32 ? 2 : 1); ++u) {
+          v[i][u] = make_uint4(0, 0, 0, 0);
+          if (in) {
+            v[i][u] = from[u];
+          }
         }
-        *reinterpret_cast<uint4 *>(to)        = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
-      } else {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (in) {
-          v = *reinterpret_cast<const uint4 *>(static_cast<const __half *>(a.q) + at_q);
+      }
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int it = threadIdx.x + (i0_ + i) * kSoftWarps * 32, part = it / (128 * CH), r = it / CH % 128, c = it % CH;
+        uint8_t  *to = sQ + part * TILE + chunk_at(r, c);
+        if constexpr (F32) {
+          float f[8] = { __uint_as_float(v[i][0].x), __uint_as_float(v[i][0].y), __uint_as_float(v[i][0].z), __uint_as_float(v[i][0].w),
+                         __uint_as_float(v[i][1].x), __uint_as_float(v[i][1].y), __uint_as_float(v[i][1].z), __uint_as_float(v[i][1].w) };
+          float m    = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            m = fmaxf(m, fabsf(f[e]));
+          }
+#pragma unroll
+          for (int o = CH / 2; o > 0; o >>= 1) {  // (CH lanes hold a row)
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          }
+          float unit, by;
+          query_unit(m, unit, by);
+          if (c == 0) {
+            bar->unit[r] = unit;
+          }
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            split_h2(f[2 * e] * by, f[2 * e + 1] * by, h[e], l[e]);
+          }
+          *reinterpret_cast<uint4 *>(to)        = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4 *>(to + TILE) = make_uint4(l[0], l[1], l[2], l[3]);
+        } else {
+          *reinterpret_cast<uint4 *>(to) = v[i][0];
         }
-        *reinterpret_cast<uint4 *>(to) = v;
       }
     }
     fence_proxy_async_smem();
@@ -228,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     const uint32_t lanes = (uint32_t) ((warp & 3) * 32) << 16;
     const uint32_t s_addr = s_at(x) + lanes, o_addr = o_at(x) + lanes;
     float          mx = kFloor, l = 0.f;
+    bool           huge = false;
     for (int j = 0; j < n_of[x] && ok; ++j) {
       const int    t    = ROWS ? j : 2 * j + x;
       const int    key0 = (first_tile + t) * kKeys;
@@ -237,86 +251,116 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       }
       tc_fence_after();
       const bool full = __all_sync(0xffffffffu, key0 >= first && key0 + kKeys - 1 <= last);
-      // ---- the row's largest score of this tile
-      float top = kFloor;
-      uint32_t s[32];
+      uint32_t s[2][32];
+      tmem_ld32_issue(s_addr, s[0]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld32_issue(s_addr + 32 * c, s);
-        tmem_ld_wait32(s);
+      for (int c = 0; c < 4; ++c) {  // 32 keys at a time, the next scores fetched under their weights
+        uint32_t(&v)[32] = s[c & 1];
+        tmem_ld_wait32(v);
         if (!full) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const int key = key0 + 32 * c + e;
-            s[e] = key <= last && key >= first ? s[e] : 0xff800000u;
+            v[e]          = key <= last && key >= first ? v[e] : 0xff800000u;
           }
         }
+        float by[2], off[2], most[2], top = -INFINITY;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float m = __uint_as_float(s[16 * h]);
+          float m0 = __uint_as_float(v[16 * h]), m1 = __uint_as_float(v[16 * h + 1]);
 #pragma unroll
-          for (int e = 1; e < 16; ++e) {
-            m = fmaxf(m, __uint_as_float(s[16 * h + e]));
+          for (int e = 2; e < 14; e += 4) {
+            m0 = max3(m0, __uint_as_float(v[16 * h + e]), __uint_as_float(v[16 * h + e + 1]));
+            m1 = max3(m1, __uint_as_float(v[16 * h + e + 2]), __uint_as_float(v[16 * h + e + 3]));
           }
-          top = fmaxf(top, fmaf(m, by_[2 * c + h] * unit, up_[2 * c + h]));
+          m0      = max3(m0, __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
+          most[h] = fmaxf(m0, m1);
+          by[h]   = by_[2 * c + h] * unit;
+          off[h]  = up_[2 * c + h] - mx + kLift;
+          top     = fmaxf(top, huge ? fmaf(most[h], by[h], up_[2 * c + h]) - mx + kLift : fmaf(most[h], by[h], off[h]));
         }
-      }
-      if (__any_sync(0xffffffffu, top > mx + kSlack)) {
-        const float m = fmaxf(mx, top), f = exp2_approx(mx - m);
-        mx = m;
-        l *= f;
-        if (j > 0) {
-          if (!(ok = wait(&bar->o_done[x], (j - 1) & 1))) {
-            break;
-          }
-          tc_fence_after();
+        if (__any_sync(0xffffffffu, top > kLift + kSlack)) {
+          // ---- a row's maximum has moved away: M follows by a power of two (exact for what is there already;
+          // straight to the maximum when nothing is)
+          const float x0 = fmaxf(fmaf(most[0], by[0], up_[2 * c]), fmaf(most[1], by[1], up_[2 * c + 1]));
+          // (first on a grid of 1 / 256, so that adding whole numbers is exact)
+          const float m  = mx == kFloor ? fmaxf(ceilf(x0 * 256.f) * 0.00390625f, kFloor) : mx + fmaxf(ceilf(x0 - mx), 0.f);
+          const int   k  = __float2int_rn(fminf(m - mx, 127.f));
+          const float f  = __int_as_float((127 - k) << 23);  // (2^-127 and less: 0)
+          mx = m;
+          l *= f;
+          off[0] = up_[2 * c] - mx + kLift, off[1] = up_[2 * c + 1] - mx + kLift;
+          huge = __any_sync(0xffffffffu, fabsf(mx) > kHuge && mx != kFloor);
+          uint32_t w[16];
+          if (c > 0) {  // weights of this tile's earlier keys
+            tmem_st_wait();
+            for (int d = 0; d < 2 * c; ++d) {
+              if (!F32 && (d & 1)) {
+                continue;  // (no second terms)
+              }
+              tmem_ld16_issue(s_addr + 16 * d, w);
+              tmem_ld_wait(w);
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            tmem_ld32_issue(o_addr + 32 * c, s);
-            tmem_ld_wait32(s);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              s[e] = __float_as_uint(__uint_as_float(s[e]) * f);
+              for (int e = 0; e < 16; ++e) {
+                const float2 u = __half22float2(u32_as_h2(w[e]));
+                w[e]           = pack_h2(u.x * f, u.y * f);
+              }
+              tmem_st16(s_addr + 16 * d, w);
             }
-            tmem_st32(o_addr + 32 * c, s);
+          }
+          if (j > 0) {
+            if (!(ok = wait(&bar->o_done[x], (j - 1) & 1))) {
+              break;
+            }
+            tc_fence_after();
+            for (int d = 0; d < D / 16; ++d) {
+              tmem_ld16_issue(o_addr + 16 * d, w);
+              tmem_ld_wait(w);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+              }
+              tmem_st16(o_addr + 16 * d, w);
+            }
           }
         }
-      }
-      // ---- weights, over the scores: 32 keys in the first 16 of their 32 columns, second terms in the others
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld32_issue(s_addr + 32 * c, s);
-        tmem_ld_wait32(s);
-        if (!full) {
+        if (huge) {  // (see kHuge)
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const int key = key0 + 32 * c + e;
-            s[e] = key <= last && key >= first ? s[e] : 0xff800000u;
+            v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), by[e >> 4], up_[2 * c + (e >> 4)]) - mx + kLift);
           }
+          by[0] = by[1] = 1.f, off[0] = off[1] = 0.f;
         }
+        if (c < 3) {
+          tmem_ld32_issue(s_addr + 32 * (c + 1), s[(c + 1) & 1]);
+        }
+        // ---- weights, over the scores: 32 keys in the first 16 of their 32 columns, second terms in the others
         uint32_t p[16], p2[16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float by = by_[2 * c + h] * unit, up = up_[2 * c + h] - mx + kLift;
-          float       sum = 0.f;
+          const float2 b2 = make_float2(by[h], by[h]), o2 = make_float2(off[h], off[h]);
+          float2       sum[2];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
-            const float u = weight_of(fmaf(__uint_as_float(s[16 * h + e]), by, up));
-            const float v = weight_of(fmaf(__uint_as_float(s[16 * h + e + 1]), by, up));
-            sum += u;
-            sum += v;
+            float2 w = fma2(make_float2(__uint_as_float(v[16 * h + e]), __uint_as_float(v[16 * h + e + 1])), b2, o2);
+            w.x = exp2_approx(w.x), w.y = exp2_approx(w.y);
+            sum[(e >> 1) & 1] = e < 4 ? w : add2(sum[(e >> 1) & 1], w);
             if constexpr (F32) {
-              split_h2(u, v, p[8 * h + e / 2], p2[8 * h + e / 2]);
+              split_h2(w.x, w.y, p[8 * h + e / 2], p2[8 * h + e / 2]);
             } else {
-              p[8 * h + e / 2] = pack_h2(u, v);
+              p[8 * h + e / 2] = pack_h2(w.x, w.y);
             }
           }
-          l = fmaf(sum, inv_[2 * c + h], l);
+          const float2 both = add2(sum[0], sum[1]);
+          l                 = fmaf(both.x + both.y, inv_[2 * c + h], l);
         }
         tmem_st16(s_addr + 32 * c, p);
         if constexpr (F32) {
           tmem_st16(s_addr + 32 * c + 16, p2);
         }
+      }
+      if (!ok) {
+        break;
       }
       tmem_st_wait();
       tc_fence_before();
@@ -347,7 +391,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       const bool part = a.groups > 1;
       const float scale = part ? 1.f : (l > 0.f ? 1.f / l : 0.f);
       float      *to = part ? a.part + ((((long long) grp * kv.n_seqs + b) * a.max_q + my_q) * a.n_heads + h) * (D + 4) : nullptr;
-      const long long at_o = (long long) (q0 + my_q) * a.out_stride + h * D;
+      // bytes of a row that this warp stages: all of it, or its stream's half of the columns
+      constexpr int ROWB  = (ROWS ? D : D / 2) * (F32 ? 4 : 2);
+      uint8_t      *stage = sQ + (warp * 32) * ROWB;
+      constexpr int SWZ = ROWB / 16 < 8 ? ROWB / 16 - 1 : 7;
+      static_assert(kSoftWarps * 32 * ROWB <= 2 * TILE, "the query parts hold the results");
       if (part && mine && (ROWS || x == 0)) {
         *reinterpret_cast<float2 *>(to + D) = make_float2(mx, l);
       }
@@ -376,22 +424,43 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
             }
           }
         }
-        if (!mine) {
-        } else if (part || F32) {
-          float *dst = part ? to + 32 * c : static_cast<float *>(a.out) + at_o + 32 * c;
+        if (part) {
+          if (mine) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            *reinterpret_cast<float4 *>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; e += 4) {
+              *reinterpret_cast<float4 *>(to + 32 * c + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            }
           }
         } else {
-          __half *dst = static_cast<__half *>(a.out) + at_o + 32 * c;
+          // to the warp's rows of the (no longer needed) query parts, 16-byte chunks swizzled by the row
+          uint8_t *srow = stage + lane * ROWB;
+          constexpr int PER = F32 ? 4 : 8;
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            *reinterpret_cast<uint4 *>(dst + e) = make_uint4(pack_h2(v[e], v[e + 1]), pack_h2(v[e + 2], v[e + 3]),
-                                                             pack_h2(v[e + 4], v[e + 5]), pack_h2(v[e + 6], v[e + 7]));
+          for (int e = 0; e < 32; e += PER) {
+            uint4 u;
+            if constexpr (F32) {
+              u = make_uint4(__float_as_uint(v[e]), __float_as_uint(v[e + 1]), __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3]));
+            } else {
+              u = make_uint4(pack_h2(v[e], v[e + 1]), pack_h2(v[e + 2], v[e + 3]), pack_h2(v[e + 4], v[e + 5]), pack_h2(v[e + 6], v[e + 7]));
+            }
+            const int chunk = (32 * k + e) / PER;
+            *reinterpret_cast<uint4 *>(srow + ((chunk ^ (lane & SWZ)) << 4)) = u;
           }
         }
         __syncwarp();  // (the next tensor-memory load is the whole warp's)
+      }
+      if (!part) {  // rows leave as contiguous runs
+        constexpr int CPR = ROWB / 16;  // chunks of a row
+#pragma unroll
+        for (int k = 0; k < CPR; ++k) {
+          const int i = k * 32 + lane, r = i / CPR, chunk = i % CPR, gr = (warp & 3) * 32 + r;
+          const int q = i0 + (ROWS ? x * per_tile : 0) + gr / a.group;
+          if (gr < per_tile * a.group && q < i1) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * ROWB + ((chunk ^ (r & SWZ)) << 4));
+            const long long at_o = (long long) (q0 + q) * a.out_stride + (head * a.group + gr % a.group) * D;
+            *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + at_o * (F32 ? 4 : 2) + (ROWS ? 0 : x * ROWB) + chunk * 16) = u;
+          }
+        }
       }
     }
     tc_fence_before();
@@ -451,42 +520,52 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         mbar_arrive(full);
       }
     };
+    // Everything of tile t + 1 is asked for before tile t + 1 is waited for: its page numbers and scales while
+    // tile t is converted, its keys (values) as soon as tile t's have left the registers.
     uint4 rk[LOADS], rv[LOADS];
-    int   pg[2] = { page_of(0, 0), page_of(0, 1) }, pn[2];
+    int   pg[2] = { page_of(0, 0), page_of(0, 1) };
+    float ks = 0.f, vs = 0.f;  // lanes 0, 1: scales of the warp's blocks; a negative one: no block
+    auto  scales = [&]() {
+      const int p = lane == 0 ? pg[0] : pg[1];
+      ks = vs = -1.f;
+      if (lane < 2 && p >= 0) {
+        ks = fmaxf(kv.k_scale[(long long) p * kv.n_kv_heads + head], 0.f);
+        vs = fmaxf(kv.v_scale[(long long) p * kv.n_kv_heads + head], 0.f);
+      }
+    };
     load(kv.k_codes, 0, pg, rk);
+    load(kv.v_codes, 0, pg, rv);
+    scales();
     bool ok = true;
     for (int t = 0; t < n && ok; ++t) {
       const int      i = t & 1;
       const uint32_t parity = ((t >> 1) & 1) ^ 1;
-      load(kv.v_codes, t, pg, rv);
-      float by = a.scale_log2, up = -INFINITY, inv = 0.f;
-      const int p = lane == 0 ? pg[0] : pg[1];
-      if (lane < 2 && p >= 0) {
-        const float ks = kv.k_scale[(long long) p * kv.n_kv_heads + head], vs = kv.v_scale[(long long) p * kv.n_kv_heads + head];
-        const float v = vs > 0.f ? vs : 1.f;
-        by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = log2f(v), inv = 1.f / v;
-      }
-      pn[0] = page_of(t + 1, 0), pn[1] = page_of(t + 1, 1);
+      const float    ks_t = ks, vs_t = vs;
+      pg[0] = page_of(t + 1, 0), pg[1] = page_of(t + 1, 1);
       if (!(ok = wait(&bar->k_empty[i], parity))) {
         break;
       }
       if (lane < 2) {
-        bar->by[t % kScaleRing][2 * cw + lane] = by, bar->up[t % kScaleRing][2 * cw + lane] = up;
-        bar->inv[t % kScaleRing][2 * cw + lane] = inv;
+        const int   at_b = 2 * cw + lane;
+        const float v    = vs_t > 0.f ? vs_t : 1.f;
+        bar->by[t % kScaleRing][at_b]  = (ks_t > 0.f ? ks_t : 1.f) * a.scale_log2;
+        bar->up[t % kScaleRing][at_b]  = vs_t < 0.f ? -INFINITY : log2f(v);
+        bar->inv[t % kScaleRing][at_b] = vs_t < 0.f ? 0.f : 1.f / v;
       }
       convert(sK + i * TILE, rk);
       publish(&bar->k_full[i]);
-      if (t + 1 < n) {
-        load(kv.k_codes, t + 1, pn, rk);
-      }
+      load(kv.k_codes, t + 1, pg, rk);
+      scales();
       if (!(ok = wait(&bar->v_empty[i], parity))) {
         break;
       }
       convert(sV + i * TILE, rv);
       publish(&bar->v_full[i]);
-      pg[0] = pn[0], pg[1] = pn[1];
+      load(kv.v_codes, t + 1, pg, rv);
     }
   } else {
+  }
+  if (warp == kMmaWarp) {
     // ---------------- MMA issuer: the whole warp walks the loop, one elected lane issues
     constexpr uint32_t IDESC_S = instr_desc_f16(128, kKeys), IDESC_O = instr_desc_f16(128, D) | kInstrBMajorMn;
     bool ok = n == 0 || wait(&bar->q_full, 0);
