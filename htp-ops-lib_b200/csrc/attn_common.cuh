@@ -3,7 +3,6 @@
 #pragma once
 
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "decoder_common.cuh"
 #include "unpack.cuh"
@@ -24,10 +23,10 @@ __device__ __forceinline__ void codes_to_h2(uint32_t w, uint32_t (&h)[2]) {
   if constexpr (KVT == kKvI8) {
     q8_0_unpack_word(w, h);
   } else {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w & 0xffff), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t) (w >> 16), __NV_E4M3);
-    h[0]                = (uint32_t) a.x | (uint32_t) a.y << 16;
-    h[1]                = (uint32_t) b.x | (uint32_t) b.y << 16;
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(h[0]), "=r"(h[1])
+        : "r"(w));
   }
 }
 

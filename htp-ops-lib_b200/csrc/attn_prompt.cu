@@ -22,7 +22,6 @@
 // issuer and tensor-memory owner.  All waits are bounded; one that runs out records error 311, raises the abort
 // flag, and every role leaves.
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "attn_common.cuh"
 #include "ptx.cuh"
@@ -41,7 +40,7 @@ constexpr int kKeys      = 128;  // keys of a tile
 constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more than a softmax warp may lag behind
 
 struct Bars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
+  uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
   uint32_t tmem;
   int      abort_flag;
   float    by[kScaleRing][8], up[kScaleRing][8], inv[kScaleRing][8];  // of the tile's 16-key blocks
@@ -147,8 +146,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     mbar_init(&bar->drained, 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 4), mbar_init(&bar->k_empty[i], 1);
-      mbar_init(&bar->v_full[i], 4), mbar_init(&bar->v_empty[i], 1);
+      mbar_init(&bar->k_full[i], 4), mbar_init(&bar->v_full[i], 4);
+      mbar_init(&bar->k_empty[i], 1), mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 2), mbar_init(&bar->p_ready[i], 4), mbar_init(&bar->o_done[i], 1);
     }
     bar->abort_flag = 0;
@@ -253,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       const bool full = __all_sync(0xffffffffu, key0 >= first && key0 + kKeys - 1 <= last);
       uint32_t s[2][32];
       tmem_ld32_issue(s_addr, s[0]);
-#pragma unroll
+#pragma unroll 2
       for (int c = 0; c < 4; ++c) {  // 32 keys at a time, the next scores fetched under their weights
         uint32_t(&v)[32] = s[c & 1];
         tmem_ld_wait32(v);
@@ -486,31 +485,53 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       }
       return p;
     };
+    constexpr int HALF = LOADS / 2;  // loads of a block
+    const int     lane_at = sub * D + piece * 16;
     auto load = [&](const uint8_t *codes, int t, const int (&pg)[2], uint4 (&r)[LOADS]) {
+      const int key0 = (first_tile + t) * kKeys + cw * 32;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int k = i * RPL + sub, key = (first_tile + t) * kKeys + cw * 32 + k, p = pg[i >= LOADS / 2];
-        r[i] = make_uint4(0, 0, 0, 0);  // (zeros behind the context: what lies there may be no numbers)
-        if (p >= 0 && key < hi && key >= lo) {
-          r[i] = ld_stream16(codes + ((((long long) p * kv.n_kv_heads + head) << kv.page_shift) + (key & (kv.page_size - 1))) * D + piece * 16);
+      for (int h = 0; h < 2; ++h) {
+        const int      key  = key0 + 16 * h;
+        const uint8_t *from = codes + ((((long long) pg[h] * kv.n_kv_heads + head) << kv.page_shift) + (key & (kv.page_size - 1))) * D + lane_at;
+        if (pg[h] >= 0 && key >= lo && key + 16 <= hi) {
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            r[h * HALF + i] = ld_stream16(from + i * RPL * D);
+          }
+        } else {  // zeros outside what any row sees: what lies there may be no numbers
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            const int k = key + i * RPL + sub;
+            r[h * HALF + i] = make_uint4(0, 0, 0, 0);
+            if (pg[h] >= 0 && k >= lo && k < hi) {
+              r[h * HALF + i] = ld_stream16(from + i * RPL * D);
+            }
+          }
         }
       }
     };
+    // where the lane's two chunks of its keys go (the swizzle takes the row modulo 8: with 4 keys a load, two
+    // cases); the upper half of a 128-element key's pieces stores its chunks in the other order: no two lanes
+    // of a row on one bank
+    const int swap = D == 128 ? piece >> 2 : 0;
+    uint32_t  put[2][2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int k = cw * 32 + e * RPL + sub;
+      put[e][0]   = chunk_at(k, 2 * piece + swap) - e * RPL * 128;
+      put[e][1]   = chunk_at(k, 2 * piece + 1 - swap) - e * RPL * 128;
+    }
     auto convert = [&](uint8_t *tile, const uint4 (&r)[LOADS]) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int      k = cw * 32 + i * RPL + sub;
         const uint32_t w[4] = { r[i].x, r[i].y, r[i].z, r[i].w };
         uint32_t       h[4][2];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          codes_to_h2<KVT>(w[e], h[e]);
+          codes_to_h2<KVT>(swap ? w[e ^ 2] : w[e], h[e]);
         }
-        const uint4 c0 = make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]), c1 = make_uint4(h[2][0], h[2][1], h[3][0], h[3][1]);
-        // (the upper half of a key's pieces stores its chunks in the other order: no two lanes of a row on one bank)
-        const int swap = D == 128 ? piece >> 2 : 0;
-        *reinterpret_cast<uint4 *>(tile + chunk_at(k, 2 * piece + swap))     = swap ? c1 : c0;
-        *reinterpret_cast<uint4 *>(tile + chunk_at(k, 2 * piece + 1 - swap)) = swap ? c0 : c1;
+        *reinterpret_cast<uint4 *>(tile + put[i & 1][0] + i * RPL * 128) = make_uint4(h[0][0], h[0][1], h[1][0], h[1][1]);
+        *reinterpret_cast<uint4 *>(tile + put[i & 1][1] + i * RPL * 128) = make_uint4(h[2][0], h[2][1], h[3][0], h[3][1]);
       }
     };
     auto publish = [&](uint64_t *full) {
@@ -538,11 +559,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     scales();
     bool ok = true;
     for (int t = 0; t < n && ok; ++t) {
-      const int      i = t & 1;
+      // Tile t - 2 has left this slot when the scores made of its keys, and the results made of its values, are
+      // complete.  KEYS: tile t / 2 - 1 of the slot's own stream, whose barriers say so.  ROWS: of both streams; the
+      // barriers of one could be two phases on by now, so the slot has its own.
+      const int      i      = t & 1;
       const uint32_t parity = ((t >> 1) & 1) ^ 1;
       const float    ks_t = ks, vs_t = vs;
       pg[0] = page_of(t + 1, 0), pg[1] = page_of(t + 1, 1);
-      if (!(ok = wait(&bar->k_empty[i], parity))) {
+      if (!(ok = t < 2 || wait(ROWS ? &bar->k_empty[i] : &bar->s_full[i], parity))) {
         break;
       }
       if (lane < 2) {
@@ -556,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       publish(&bar->k_full[i]);
       load(kv.k_codes, t + 1, pg, rk);
       scales();
-      if (!(ok = wait(&bar->v_empty[i], parity))) {
+      if (!(ok = t < 2 || wait(ROWS ? &bar->v_empty[i] : &bar->o_done[i], parity))) {
         break;
       }
       convert(sV + i * TILE, rv);
@@ -591,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         }
         umma_commit<false>(&bar->s_full[x]);
         mbar_arrive(&bar->s_full[x]);  // (carries the converters' scales on to the softmax warps)
-        if (!ROWS || x == 1) {
+        if (ROWS && x == 1) {
           umma_commit<false>(&bar->k_empty[i]);
         }
       }
@@ -628,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
             }
           }
           umma_commit<false>(&bar->o_done[x]);
-          if (!ROWS || x == 1) {
+          if (ROWS && x == 1) {
             umma_commit<false>(&bar->v_empty[i]);
           }
         }
