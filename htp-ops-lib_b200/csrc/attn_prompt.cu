@@ -93,7 +93,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
   constexpr int TILE  = Sizes<D>::kTile;
   constexpr int TERMS = F32 ? 2 : 1;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t) 1023);
+  // (an offset, not a rounded address: the compiler keeps seeing shared memory)
+  uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
   uint8_t *sQ = smem, *sK = smem + 2 * TILE, *sV = smem + 4 * TILE;
   Bars    *bar = reinterpret_cast<Bars *>(smem + 6 * TILE);
   pdl_launch_dependents();
