@@ -242,6 +242,42 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     const uint32_t s_addr = s_at(x) + lanes, o_addr = o_at(x) + lanes;
     float          mx = kFloor, l = 0.f;
     bool           huge = false;
+    // multiplies what a row has by f: the weights of this tile's first c chunks of 32 keys and, from the second
+    // tile on, O
+    auto rescale = [&](int j, int c, float f) {
+      uint32_t w[16];
+      if (c > 0) {
+        tmem_st_wait();
+#pragma unroll 1
+        for (int d = 0; d < 2 * c; d += F32 ? 1 : 2) {
+          tmem_ld16_issue(s_addr + 16 * d, w);
+          tmem_ld_wait(w);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 u = __half22float2(u32_as_h2(w[e]));
+            w[e]           = pack_h2(u.x * f, u.y * f);
+          }
+          tmem_st16(s_addr + 16 * d, w);
+        }
+      }
+      if (j > 0) {
+        if (!wait(&bar->o_done[x], (j - 1) & 1)) {
+          return false;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int d = 0; d < D / 16; ++d) {
+          tmem_ld16_issue(o_addr + 16 * d, w);
+          tmem_ld_wait(w);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+          }
+          tmem_st16(o_addr + 16 * d, w);
+        }
+      }
+      return true;
+    };
     for (int j = 0; j < n_of[x] && ok; ++j) {
       const int    t    = ROWS ? j : 2 * j + x;
       const int    key0 = (first_tile + t) * kKeys;
@@ -251,112 +287,102 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       }
       tc_fence_after();
       const bool full = __all_sync(0xffffffffu, key0 >= first && key0 + kKeys - 1 <= last);
+      // 64 keys at a time; the registers of 32 are filled with later scores as soon as their weights are made
       uint32_t s[2][32];
       tmem_ld32_issue(s_addr, s[0]);
-#pragma unroll 2
-      for (int c = 0; c < 4; ++c) {  // 32 keys at a time, the next scores fetched under their weights
-        uint32_t(&v)[32] = s[c & 1];
-        tmem_ld_wait32(v);
+      tmem_ld32_issue(s_addr + 32, s[1]);
+#pragma unroll 1
+      for (int c = 0; c < 4 && ok; c += 2) {
+        tmem_ld_wait32(s[0]);
+        tmem_ld_wait32(s[1]);
         if (!full) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int key = key0 + 32 * c + e;
-            v[e]          = key <= last && key >= first ? v[e] : 0xff800000u;
+          for (int e = 0; e < 64; ++e) {
+            const int key     = key0 + 32 * c + e;
+            s[e >> 5][e & 31] = key <= last && key >= first ? s[e >> 5][e & 31] : 0xff800000u;
           }
         }
-        float by[2], off[2], most[2], top = -INFINITY;
+        float by[4], up[4], off[4], most[4], top = -INFINITY;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float m0 = __uint_as_float(v[16 * h]), m1 = __uint_as_float(v[16 * h + 1]);
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t *v = s[h >> 1] + 16 * (h & 1);
+          float m0 = __uint_as_float(v[0]), m1 = __uint_as_float(v[1]);
 #pragma unroll
           for (int e = 2; e < 14; e += 4) {
-            m0 = max3(m0, __uint_as_float(v[16 * h + e]), __uint_as_float(v[16 * h + e + 1]));
-            m1 = max3(m1, __uint_as_float(v[16 * h + e + 2]), __uint_as_float(v[16 * h + e + 3]));
+            m0 = max3(m0, __uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            m1 = max3(m1, __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3]));
           }
-          m0      = max3(m0, __uint_as_float(v[16 * h + 14]), __uint_as_float(v[16 * h + 15]));
+          m0      = max3(m0, __uint_as_float(v[14]), __uint_as_float(v[15]));
           most[h] = fmaxf(m0, m1);
           by[h]   = by_[2 * c + h] * unit;
-          off[h]  = up_[2 * c + h] - mx + kLift;
-          top     = fmaxf(top, huge ? fmaf(most[h], by[h], up_[2 * c + h]) - mx + kLift : fmaf(most[h], by[h], off[h]));
+          up[h]   = up_[2 * c + h];
+          off[h]  = up[h] - mx + kLift;
+          top     = fmaxf(top, huge ? fmaf(most[h], by[h], up[h]) - mx + kLift : fmaf(most[h], by[h], off[h]));
         }
         if (__any_sync(0xffffffffu, top > kLift + kSlack)) {
           // ---- a row's maximum has moved away: M follows by a power of two (exact for what is there already;
           // straight to the maximum when nothing is)
-          const float x0 = fmaxf(fmaf(most[0], by[0], up_[2 * c]), fmaf(most[1], by[1], up_[2 * c + 1]));
+          float x0 = fmaf(most[0], by[0], up[0]);
+#pragma unroll
+          for (int h = 1; h < 4; ++h) {
+            x0 = fmaxf(x0, fmaf(most[h], by[h], up[h]));
+          }
           // (first on a grid of 1 / 256, so that adding whole numbers is exact)
-          const float m  = mx == kFloor ? fmaxf(ceilf(x0 * 256.f) * 0.00390625f, kFloor) : mx + fmaxf(ceilf(x0 - mx), 0.f);
-          const int   k  = __float2int_rn(fminf(m - mx, 127.f));
-          const float f  = __int_as_float((127 - k) << 23);  // (2^-127 and less: 0)
+          const float m = mx == kFloor ? fmaxf(ceilf(x0 * 256.f) * 0.00390625f, kFloor) : mx + fmaxf(ceilf(x0 - mx), 0.f);
+          const int   k = __float2int_rn(fminf(m - mx, 127.f));
+          const float f = __int_as_float((127 - k) << 23);  // (2^-127 and less: 0)
           mx = m;
           l *= f;
-          off[0] = up_[2 * c] - mx + kLift, off[1] = up_[2 * c + 1] - mx + kLift;
-          huge = __any_sync(0xffffffffu, fabsf(mx) > kHuge && mx != kFloor);
-          uint32_t w[16];
-          if (c > 0) {  // weights of this tile's earlier keys
-            tmem_st_wait();
-            for (int d = 0; d < 2 * c; ++d) {
-              if (!F32 && (d & 1)) {
-                continue;  // (no second terms)
-              }
-              tmem_ld16_issue(s_addr + 16 * d, w);
-              tmem_ld_wait(w);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float2 u = __half22float2(u32_as_h2(w[e]));
-                w[e]           = pack_h2(u.x * f, u.y * f);
-              }
-              tmem_st16(s_addr + 16 * d, w);
-            }
+          for (int h = 0; h < 4; ++h) {
+            off[h] = up[h] - mx + kLift;
           }
-          if (j > 0) {
-            if (!(ok = wait(&bar->o_done[x], (j - 1) & 1))) {
-              break;
-            }
-            tc_fence_after();
-            for (int d = 0; d < D / 16; ++d) {
-              tmem_ld16_issue(o_addr + 16 * d, w);
-              tmem_ld_wait(w);
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                w[e] = __float_as_uint(__uint_as_float(w[e]) * f);
-              }
-              tmem_st16(o_addr + 16 * d, w);
-            }
+          huge = __any_sync(0xffffffffu, fabsf(mx) > kHuge && mx != kFloor);
+          ok   = rescale(j, c, f);
+          if (!ok) {
+            break;
           }
         }
         if (huge) {  // (see kHuge)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), by[e >> 4], up_[2 * c + (e >> 4)]) - mx + kLift);
+          for (int e = 0; e < 64; ++e) {
+            uint32_t &v = s[e >> 5][e & 31];
+            v = __float_as_uint(fmaf(__uint_as_float(v), by[e >> 4], up[e >> 4]) - mx + kLift);
           }
-          by[0] = by[1] = 1.f, off[0] = off[1] = 0.f;
-        }
-        if (c < 3) {
-          tmem_ld32_issue(s_addr + 32 * (c + 1), s[(c + 1) & 1]);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            by[h] = 1.f, off[h] = 0.f;
+          }
         }
         // ---- weights, over the scores: 32 keys in the first 16 of their 32 columns, second terms in the others
-        uint32_t p[16], p2[16];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 b2 = make_float2(by[h], by[h]), o2 = make_float2(off[h], off[h]);
-          float2       sum[2];
+        for (int d = 0; d < 2; ++d) {
+          uint32_t p[16], p2[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float2 w = fma2(make_float2(__uint_as_float(v[16 * h + e]), __uint_as_float(v[16 * h + e + 1])), b2, o2);
-            w.x = exp2_approx(w.x), w.y = exp2_approx(w.y);
-            sum[(e >> 1) & 1] = e < 4 ? w : add2(sum[(e >> 1) & 1], w);
-            if constexpr (F32) {
-              split_h2(w.x, w.y, p[8 * h + e / 2], p2[8 * h + e / 2]);
-            } else {
-              p[8 * h + e / 2] = pack_h2(w.x, w.y);
+          for (int h = 0; h < 2; ++h) {
+            const float2 b2 = make_float2(by[2 * d + h], by[2 * d + h]), o2 = make_float2(off[2 * d + h], off[2 * d + h]);
+            float2       sum[2];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float2 w = fma2(make_float2(__uint_as_float(s[d][16 * h + e]), __uint_as_float(s[d][16 * h + e + 1])), b2, o2);
+              w.x = exp2_approx(w.x), w.y = exp2_approx(w.y);
+              sum[(e >> 1) & 1] = e < 4 ? w : add2(sum[(e >> 1) & 1], w);
+              if constexpr (F32) {
+                split_h2(w.x, w.y, p[8 * h + e / 2], p2[8 * h + e / 2]);
+              } else {
+                p[8 * h + e / 2] = pack_h2(w.x, w.y);
+              }
             }
+            const float2 both = add2(sum[0], sum[1]);
+            l                 = fmaf(both.x + both.y, inv_[2 * (c + d) + h], l);
           }
-          const float2 both = add2(sum[0], sum[1]);
-          l                 = fmaf(both.x + both.y, inv_[2 * c + h], l);
-        }
-        tmem_st16(s_addr + 32 * c, p);
-        if constexpr (F32) {
-          tmem_st16(s_addr + 32 * c + 16, p2);
+          if (c == 0) {
+            tmem_ld32_issue(s_addr + 32 * (2 + d), s[d]);
+          }
+          tmem_st16(s_addr + 32 * (c + d), p);
+          if constexpr (F32) {
+            tmem_st16(s_addr + 32 * (c + d) + 16, p2);
+          }
         }
       }
       if (!ok) {
@@ -542,51 +568,62 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         mbar_arrive(full);
       }
     };
-    // Everything of tile t + 1 is asked for before tile t + 1 is waited for: its page numbers and scales while
-    // tile t is converted, its keys (values) as soon as tile t's have left the registers.
+    // Keys go one tile ahead of values: the next scores are wanted before this tile's results.  Loads are in
+    // flight for a tile's time: a tile's page numbers and scales, then its keys and values, are asked for
+    // when the registers of the tile before have been converted.
     uint4 rk[LOADS], rv[LOADS];
-    int   pg[2] = { page_of(0, 0), page_of(0, 1) };
+    int   pk[2] = { page_of(0, 0), page_of(0, 1) }, pv[2] = { pk[0], pk[1] };
     float ks = 0.f, vs = 0.f;  // lanes 0, 1: scales of the warp's blocks; a negative one: no block
     auto  scales = [&]() {
-      const int p = lane == 0 ? pg[0] : pg[1];
+      const int p = lane == 0 ? pk[0] : pk[1];
       ks = vs = -1.f;
       if (lane < 2 && p >= 0) {
         ks = fmaxf(kv.k_scale[(long long) p * kv.n_kv_heads + head], 0.f);
         vs = fmaxf(kv.v_scale[(long long) p * kv.n_kv_heads + head], 0.f);
       }
     };
-    load(kv.k_codes, 0, pg, rk);
-    load(kv.v_codes, 0, pg, rv);
+    load(kv.k_codes, 0, pk, rk);
+    load(kv.v_codes, 0, pv, rv);
     scales();
     bool ok = true;
-    for (int t = 0; t < n && ok; ++t) {
-      // Tile t - 2 has left this slot when the scores made of its keys, and the results made of its values, are
-      // complete.  KEYS: tile t / 2 - 1 of the slot's own stream, whose barriers say so.  ROWS: of both streams; the
-      // barriers of one could be two phases on by now, so the slot has its own.
+    // Slot t & 1 is free when the scores made of tile t - 2's keys, the results made of its values, are complete.
+    // KEYS: tile t / 2 - 1 of the slot's own stream, whose barriers say so.  ROWS: of both streams; the
+    // barriers of one could be two phases on by now, so the slot has its own.
+    auto keys = [&](int t) {
       const int      i      = t & 1;
       const uint32_t parity = ((t >> 1) & 1) ^ 1;
-      const float    ks_t = ks, vs_t = vs;
-      pg[0] = page_of(t + 1, 0), pg[1] = page_of(t + 1, 1);
+      const float    v      = vs > 0.f ? vs : 1.f;
+      const float    by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = vs < 0.f ? -INFINITY : log2f(v), inv = vs < 0.f ? 0.f : 1.f / v;
+      pk[0] = page_of(t + 1, 0), pk[1] = page_of(t + 1, 1);
       if (!(ok = t < 2 || wait(ROWS ? &bar->k_empty[i] : &bar->s_full[i], parity))) {
-        break;
+        return;
       }
       if (lane < 2) {
-        const int   at_b = 2 * cw + lane;
-        const float v    = vs_t > 0.f ? vs_t : 1.f;
-        bar->by[t % kScaleRing][at_b]  = (ks_t > 0.f ? ks_t : 1.f) * a.scale_log2;
-        bar->up[t % kScaleRing][at_b]  = vs_t < 0.f ? -INFINITY : log2f(v);
-        bar->inv[t % kScaleRing][at_b] = vs_t < 0.f ? 0.f : 1.f / v;
+        bar->by[t % kScaleRing][2 * cw + lane] = by, bar->up[t % kScaleRing][2 * cw + lane] = up;
+        bar->inv[t % kScaleRing][2 * cw + lane] = inv;
       }
       convert(sK + i * TILE, rk);
       publish(&bar->k_full[i]);
-      load(kv.k_codes, t + 1, pg, rk);
+      load(kv.k_codes, t + 1, pk, rk);
       scales();
-      if (!(ok = t < 2 || wait(ROWS ? &bar->v_empty[i] : &bar->o_done[i], parity))) {
+    };
+    if (n > 0) {
+      keys(0);
+    }
+#pragma unroll 1
+    for (int t = 0; t < n && ok; ++t) {
+      const int      i      = t & 1;
+      const uint32_t parity = ((t >> 1) & 1) ^ 1;
+      pv[0] = pk[0], pv[1] = pk[1];  // (of tile t + 1)
+      if (t + 1 < n) {
+        keys(t + 1);
+      }
+      if (!ok || !(ok = t < 2 || wait(ROWS ? &bar->v_empty[i] : &bar->o_done[i], parity))) {
         break;
       }
       convert(sV + i * TILE, rv);
       publish(&bar->v_full[i]);
-      load(kv.v_codes, t + 1, pg, rv);
+      load(kv.v_codes, t + 1, pv, rv);
     }
   } else {
   }
