@@ -19,7 +19,7 @@
 // (16 per cycle and SM); fp32 doubles the tensor-core part.
 //
 // Roles: warps 0-3 and 4-7 softmax of stream 0 and 1 (thread = row = TMEM lane), 8-11 converters, 12 MMA
-// issuer and tensor-memory owner.  All waits are bounded; one that runs out records error 311, raises the abort
+// issuer and tensor-memory owner, 13 scales.  All waits are bounded; one that runs out records error 311, raises the abort
 // flag, and every role leaves.
 #include <cuda_fp16.h>
 
@@ -35,7 +35,8 @@ namespace {
 constexpr int kSoftWarps = 8;
 constexpr int kConvWarp0 = 8;
 constexpr int kMmaWarp   = 12;
-constexpr int kThreads   = 16 * 32;  // warps 13-15 only lend their registers
+constexpr int kScaleWarp = 13;
+constexpr int kThreads   = 14 * 32;
 constexpr int kKeys      = 128;  // keys of a tile
 constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more than a softmax warp may lag behind
 
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     mbar_init(&bar->drained, 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar->k_full[i], 4), mbar_init(&bar->v_full[i], 4);
+      mbar_init(&bar->k_full[i], 5), mbar_init(&bar->v_full[i], 4);  // (the converters; keys: and the scales)
       mbar_init(&bar->k_empty[i], 1), mbar_init(&bar->v_empty[i], 1);
       mbar_init(&bar->s_full[i], 2), mbar_init(&bar->p_ready[i], 4), mbar_init(&bar->o_done[i], 1);
     }
@@ -163,6 +164,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&bar->tmem);
   const Waiter   wait{ &bar->abort_flag, a.err };
+  const int     *table = kv.page_table + (long long) b * kv.table_stride;
+  auto           seen  = [&](int key) { return key < hi && key + 16 > lo; };  // some row sees some of these 16 keys
+  // Slot t & 1 is free for tile t when the scores made of tile t - 2's keys, or the results made of its values,
+  // are complete.  KEYS: tile t / 2 - 1 of the slot's own stream, whose barriers say so.  ROWS: of both
+  // streams; the barriers of one could be two phases on by now, so the slots have their own.
+  auto slot_free = [&](int t, uint64_t *empty, uint64_t *own) {
+    return t < 2 || wait(ROWS ? empty + (t & 1) : own + (t & 1), ((t >> 1) & 1) ^ 1);
+  };
   auto           s_at = [&](int x) { return tmem + (uint32_t) x * 128; };
   auto           o_at = [&](int x) { return tmem + 256 + (uint32_t) x * 128; };
 
@@ -496,21 +505,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     constexpr int RPL    = 32 / PIECES;       // keys of one warp-wide load
     constexpr int LOADS  = 32 / RPL;          // loads of a lane per tile
     const int cw = warp - kConvWarp0, piece = lane % PIECES, sub = lane / PIECES;
-    const int     *table = kv.page_table + (long long) b * kv.table_stride;
-    // page of block i (0, 1) of this warp's keys in tile t; -1: nothing there, -2: a bad entry
-    auto page_of = [&](int t, int i) {
-      const int key = (first_tile + t) * kKeys + cw * 32 + 16 * i;
-      if (t >= n || key >= hi || key + 16 <= lo) {
-        return -1;
+    // page numbers of the warp's two blocks in tile t, as they stand in the table; checked when they are used
+    auto ask = [&](int t, int (&raw)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int key = (first_tile + t) * kKeys + cw * 32 + 16 * h;
+        raw[h]        = t < n && seen(key) ? table[key >> kv.page_shift] : -1;
       }
-      const int p = table[key >> kv.page_shift];
-      if (p < 0 || p >= kv.n_pages) {
-        if (lane == 0) {
-          record_error(a.err, kErrPage);
-        }
-        return -2;
+    };
+    auto checked = [&](const int (&raw)[2], int (&pg)[2]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pg[h] = raw[h] < kv.n_pages ? raw[h] : -1;  // (negative: nothing is read)
       }
-      return p;
     };
     constexpr int HALF = LOADS / 2;  // loads of a block
     const int     lane_at = sub * D + piece * 16;
@@ -569,65 +576,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       }
     };
     // Keys go one tile ahead of values: the next scores are wanted before this tile's results.  Loads are in
-    // flight for a tile's time: a tile's page numbers and scales, then its keys and values, are asked for
-    // when the registers of the tile before have been converted.
+    // flight for a tile's time: a tile's keys and values are asked for when the registers of the tile
+    // before have been converted, its page numbers a tile earlier.
     uint4 rk[LOADS], rv[LOADS];
-    int   pk[2] = { page_of(0, 0), page_of(0, 1) }, pv[2] = { pk[0], pk[1] };
-    float ks = 0.f, vs = 0.f;  // lanes 0, 1: scales of the warp's blocks; a negative one: no block
-    auto  scales = [&]() {
-      const int p = lane == 0 ? pk[0] : pk[1];
-      ks = vs = -1.f;
-      if (lane < 2 && p >= 0) {
-        ks = fmaxf(kv.k_scale[(long long) p * kv.n_kv_heads + head], 0.f);
-        vs = fmaxf(kv.v_scale[(long long) p * kv.n_kv_heads + head], 0.f);
-      }
-    };
+    int   raw[2], pk[2], pv[2];
+    ask(0, raw);
+    checked(raw, pk);
     load(kv.k_codes, 0, pk, rk);
-    load(kv.v_codes, 0, pv, rv);
-    scales();
+    load(kv.v_codes, 0, pk, rv);
+    ask(1, raw);
     bool ok = true;
-    // Slot t & 1 is free when the scores made of tile t - 2's keys, the results made of its values, are complete.
-    // KEYS: tile t / 2 - 1 of the slot's own stream, whose barriers say so.  ROWS: of both streams; the
-    // barriers of one could be two phases on by now, so the slot has its own.
     auto keys = [&](int t) {
-      const int      i      = t & 1;
-      const uint32_t parity = ((t >> 1) & 1) ^ 1;
-      const float    v      = vs > 0.f ? vs : 1.f;
-      const float    by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = vs < 0.f ? -INFINITY : log2f(v), inv = vs < 0.f ? 0.f : 1.f / v;
-      pk[0] = page_of(t + 1, 0), pk[1] = page_of(t + 1, 1);
-      if (!(ok = t < 2 || wait(ROWS ? &bar->k_empty[i] : &bar->s_full[i], parity))) {
+      const int i = t & 1;
+      if (!(ok = slot_free(t, bar->k_empty, bar->s_full))) {
         return;
-      }
-      if (lane < 2) {
-        bar->by[t % kScaleRing][2 * cw + lane] = by, bar->up[t % kScaleRing][2 * cw + lane] = up;
-        bar->inv[t % kScaleRing][2 * cw + lane] = inv;
       }
       convert(sK + i * TILE, rk);
       publish(&bar->k_full[i]);
+      checked(raw, pk);
       load(kv.k_codes, t + 1, pk, rk);
-      scales();
+      ask(t + 2, raw);
     };
     if (n > 0) {
       keys(0);
     }
 #pragma unroll 1
     for (int t = 0; t < n && ok; ++t) {
-      const int      i      = t & 1;
-      const uint32_t parity = ((t >> 1) & 1) ^ 1;
       pv[0] = pk[0], pv[1] = pk[1];  // (of tile t + 1)
       if (t + 1 < n) {
         keys(t + 1);
       }
-      if (!ok || !(ok = t < 2 || wait(ROWS ? &bar->v_empty[i] : &bar->o_done[i], parity))) {
+      if (!ok || !(ok = slot_free(t, bar->v_empty, bar->o_done))) {
         break;
       }
-      convert(sV + i * TILE, rv);
-      publish(&bar->v_full[i]);
+      convert(sV + (t & 1) * TILE, rv);
+      publish(&bar->v_full[t & 1]);
       load(kv.v_codes, t + 1, pv, rv);
     }
+  } else if (warp == kScaleWarp) {
+    // ---------------- scales of the tiles' 16-key blocks, a lane each; what is no block gets the weight 0
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+      const int key = (first_tile + t) * kKeys + 16 * (lane & 7);
+      float     by = a.scale_log2, up = -INFINITY, inv = 0.f;
+      if (seen(key)) {
+        const int p = table[key >> kv.page_shift];
+        if (p < 0 || p >= kv.n_pages) {
+          record_error(a.err, kErrPage);
+        } else {
+          const float ks = kv.k_scale[(long long) p * kv.n_kv_heads + head], vs = kv.v_scale[(long long) p * kv.n_kv_heads + head];
+          const float v  = vs > 0.f ? vs : 1.f;
+          by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = log2f(v), inv = 1.f / v;
+        }
+      }
+      __syncwarp();
+      if (!slot_free(t, bar->k_empty, bar->s_full)) {
+        break;
+      }
+      if (lane < 8) {
+        bar->by[t % kScaleRing][lane] = by, bar->up[t % kScaleRing][lane] = up, bar->inv[t % kScaleRing][lane] = inv;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar->k_full[t & 1]);
+      }
+    }
   } else {
-  }
-  if (warp == kMmaWarp) {
     // ---------------- MMA issuer: the whole warp walks the loop, one elected lane issues
     constexpr uint32_t IDESC_S = instr_desc_f16(128, kKeys), IDESC_O = instr_desc_f16(128, D) | kInstrBMajorMn;
     bool ok = n == 0 || wait(&bar->q_full, 0);
