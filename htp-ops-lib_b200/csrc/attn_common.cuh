@@ -51,6 +51,18 @@ __device__ __forceinline__ void query_unit(float amax, float &unit, float &by) {
   by    = __int_as_float((127 - e) << 23);
 }
 
+// What a block's scales become: factor of its scores, addend to its exponents, divisor of its weights in the
+// denominator.  (The logarithm of the mantissa alone: off by 2^-22 whatever the exponent.)
+__device__ __forceinline__ void block_scales(float ks, float vs, float scale_log2, float &by, float &up, float &inv) {
+  const float v = vs > 0.f ? vs : 1.f;
+  const int   e = (__float_as_int(v) >> 23) - 127;
+  float       m;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(m) : "f"(__int_as_float((__float_as_int(v) & 0x007fffff) | 0x3f800000)));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(v));
+  by = (ks > 0.f ? ks : 1.f) * scale_log2;
+  up = (float) e + m;
+}
+
 // Two fp32 operations of one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;

@@ -5,7 +5,7 @@
 // every code is fetched from HBM once and the warp-level tensor-core instructions work on full tiles:
 //   S^T[token][column] = K[token][d] . Q^T[d][column]     A = 16 tokens of codes, B = the queries
 //   O^T[d][column]    += V^T[d][token] . P^T[token][column]
-// Codes become fp16 exactly (signed bytes and e4m3 both fit) on their way from global memory to the A
+// Codes become fp16 exactly (signed bytes and e4m3 both fit) on their way from shared memory to the A
 // fragments, in registers: the order of d inside a fragment is free as long as K and Q (or V^T and O^T)
 // agree, so each lane loads 16 contiguous bytes of a row.  P^T comes from S^T by an 8 x 8 transpose in the
 // warp.  fp32 queries and weights are two fp16 terms each (hi + lo), two MMAs into the same accumulator.
@@ -15,11 +15,13 @@
 // than kSlack behind), O sums n * code, and the softmax denominator sums n / v_scale per block: one running
 // maximum, one FMA and one exponential per score, everything in fp32.
 //
-// Work: CTA = 4 warps; a warp walks 32-token steps of its CTA's share of the context, its next loads issued
-// while the current step computes.  A context is shared by the CTAs of a cluster, whose results meet in
+// Work: CTA = 4 warps; a warp walks 32-token steps of its CTA's share of the context, the next steps
+// on their way to its ring in shared memory meanwhile: tiled copies of 16 tokens (2 KB runs in
+// HBM; 64- and 128-byte pieces fetched by the lanes themselves reached 4.4 of 6.5 TB/s with nothing computed).  A context is shared by the CTAs of a cluster, whose results meet in
 // distributed shared memory in rank order; long contexts of few sequences by several clusters, whose results
 // meet in the workspace and a second small launch.  No atomics: results do not depend on scheduling.
 #include <cooperative_groups.h>
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -34,7 +36,31 @@ namespace {
 
 constexpr int   kWarps   = 4;
 constexpr int   kThreads = kWarps * 32;
-constexpr int   kStep    = 32;     // tokens of a warp's step: two 16-token MMA tiles
+constexpr int   kStep    = 32;  // tokens of a warp's step: two 16-token MMA tiles
+constexpr int   kStages  = 2;   // steps of a warp in shared memory or on their way
+// One step of a warp: two 16-token tiles of keys and of values as the copy engine lays them down, rows of D bytes
+// with their 16-byte chunks swizzled by the row (128 or 64 bytes wide).
+template <int D>
+struct alignas(1024) DecodeStage {
+  uint8_t k[2][16 * D], v[2][16 * D];
+};
+// byte offset of the 16-byte chunk c of row r
+template <int D>
+__device__ __forceinline__ int swizzled(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+// Token of MMA row (and of position k of the second product) i, 0 .. 7; rows 8 .. 15 are its tokens plus 8.
+// Rows of one 8-lane phase then differ in bits 0 and 2, the rows of one lane group in bits 1 and 2: no two
+// lanes of a phase meet on a bank, whether they read keys by rows or values by columns.
+__device__ __forceinline__ int token_of(int i) {
+  return i & 1 ? (i - 1) ^ 5 : i;
+}
+
+struct DecodeArgs {
+  AttnArgs    a;
+  CUtensorMap kmap, vmap;  // codes as rows of head_dim bytes, boxes of 16 rows
+};
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -42,7 +68,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 template <int KVT, int D, int NT, bool F32>
-__global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_constant__ DecodeArgs args) {
+  const AttnArgs &a = args.a;
   constexpr int NC    = NT * 8;
   constexpr int KI    = D / 64;          // 16-byte pieces of a key row per lane
   constexpr int MT    = D / 16;          // 16-row tiles of O^T
@@ -50,17 +77,32 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
   constexpr int TERMS = F32 ? 2 : 1;
   constexpr int QP    = D + 8;           // pitch of a query column in shared memory (halves): conflict-free 16-byte reads
   constexpr int OP    = D + 4;           // pitch of an output column (floats)
-  __shared__ __align__(16) union {
-    __half q[TERMS][NC][QP];
-    float  o[kWarps][NC][OP];
-  } sm;
+  using Stage = DecodeStage<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (the same in every CTA of a cluster)
+  Stage   *ring = reinterpret_cast<Stage *>(smem) + (threadIdx.x >> 5) * kStages;  // this warp's
+  // the warps' results take the rings' place
+  float(*sm_o)[NC][OP] = reinterpret_cast<float(*)[NC][OP]>(smem);
+  static_assert(sizeof(float) * kWarps * NC * OP <= sizeof(Stage) * kWarps * kStages, "room for the results");
+  __shared__ __align__(16) __half sm_q[TERMS][NC][QP];
   __shared__ float ml[kWarps][2][NC];
   __shared__ float q_unit[NC];  // fp32 queries: the power of two that a column was divided by
+  __shared__ uint64_t bars[kWarps][kStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars[warp][i], 1);
+    }
+    mbar_fence_init();
+    tma_prefetch_descriptor(&args.kmap);
+    tma_prefetch_descriptor(&args.vmap);
+  }
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait_prior_grids();
 
-  const KvView &kv   = a.kv;
-  const int     warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const KvView &kv = a.kv;
   unsigned      id    = blockIdx.x;
   const int     split = id % a.splits;
   id /= a.splits;
@@ -104,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       if constexpr (F32) {
         v = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.q) + at);
       } else {
-        *reinterpret_cast<uint2 *>(&sm.q[0][c][d]) = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + at);
+        *reinterpret_cast<uint2 *>(&sm_q[0][c][d]) = *reinterpret_cast<const uint2 *>(static_cast<const __half *>(a.q) + at);
         continue;
       }
     }
@@ -124,9 +166,9 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
     uint2 h, l;
     split_h2(v.x, v.y, h.x, l.x);
     split_h2(v.z, v.w, h.y, l.y);
-    *reinterpret_cast<uint2 *>(&sm.q[0][c][d]) = h;
+    *reinterpret_cast<uint2 *>(&sm_q[0][c][d]) = h;
     if constexpr (F32) {
-      *reinterpret_cast<uint2 *>(&sm.q[TERMS - 1][c][d]) = l;
+      *reinterpret_cast<uint2 *>(&sm_q[TERMS - 1][c][d]) = l;
     }
   }
   // what the lane's columns (2 t, 2 t + 1 of each 8) see: tokens first[] .. last[]
@@ -144,61 +186,48 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
 
   const int       P = kv.page_size;
   const int      *table = kv.page_table + (long long) b * kv.table_stride;
-  // page of a step's tile, -1 where there is nothing to read (outside lo .. hi, or a bad entry)
-  auto page_of = [&](int step, int tile) {
-    const int tok = step * kStep + tile * 16;
-    if (step >= end || tok >= hi || tok + 16 <= lo) {
-      return -1;
-    }
-    const int p = table[tok >> kv.page_shift];
-    if (p < 0 || p >= kv.n_pages) {
-      if (lane == 0) {
-        record_error(a.err, kErrPage);
-      }
-      return -1;
-    }
-    return p;
-  };
-  uint4    kr[2][2][KI];
-  uint32_t vr[2][4][VW];
-  float    ks[2], vs[2];
-  auto     offset = [&](int page, int step, int tile) {
-    return ((((long long) page * kv.n_kv_heads + head) << kv.page_shift) + ((step * kStep + tile * 16) & (P - 1))) * D;
-  };
-  auto load_k = [&](int step, const int (&pg)[2]) {
+  // page numbers of a step's two tiles as they stand in the table (-1 where there is nothing to read)
+  auto ask = [&](int step, int (&raw)[2]) {
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      if (pg[m] >= 0) {
-        const uint8_t *base = kv.k_codes + offset(pg[m], step, m) + g * D + t * 16;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-#pragma unroll
-          for (int i = 0; i < KI; ++i) {
-            kr[m][r][i] = ld_stream16(base + r * 8 * D + i * 64);
-          }
-        }
-        ks[m] = kv.k_scale[(long long) pg[m] * kv.n_kv_heads + head];
-      }
+      const int tok = step * kStep + m * 16;
+      raw[m]        = step < end && tok < hi && tok + 16 > lo ? table[tok >> kv.page_shift] : -1;
     }
   };
-  auto load_v = [&](int step, const int (&pg)[2]) {
+  // Asks for a step: four tiled copies on one barrier, and per lane the scales of tile lane & 1.  raw: checked
+  // on the way, -1 for a bad entry.
+  const uint64_t policy = l2_policy_evict_first();
+  auto fetch = [&](int step, int slot, int (&raw)[2], float (&scale)[2]) {
+    int tiles = 0;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      if (pg[m] >= 0) {
-        const uint8_t *base = kv.v_codes + offset(pg[m], step, m) + g * (D / 8);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-          const uint8_t *at = base + (2 * t + (r & 1) + (r >> 1) * 8) * D;
-          if constexpr (VW == 4) {
-            const uint4 v = ld_stream16(at);
-            vr[m][r][0] = v.x, vr[m][r][1] = v.y, vr[m][r][2] = v.z, vr[m][r][3] = v.w;
-          } else {
-            const uint2 v = ld_stream8(at);
-            vr[m][r][0] = v.x, vr[m][r][1] = v.y;
-          }
+      const int tok = step * kStep + m * 16;
+      if (raw[m] < 0 || raw[m] >= kv.n_pages) {
+        if (lane == 0 && step < end && tok < hi && tok + 16 > lo) {
+          record_error(a.err, kErrPage);
         }
-        vs[m] = kv.v_scale[(long long) pg[m] * kv.n_kv_heads + head];
+        raw[m] = -1;
+      } else {
+        ++tiles;
       }
+    }
+    if (lane == 0) {
+      uint64_t *bar = &bars[warp][slot];
+      mbar_arrive_expect_tx(bar, tiles * 2 * 16 * D);
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        if (raw[m] >= 0) {
+          // (the entry points see to it that a cache has fewer than 2^31 rows)
+          const int row = (((raw[m] * kv.n_kv_heads) + head) << kv.page_shift) + ((step * kStep + m * 16) & (P - 1));
+          tma_load_2d(ring[slot].k[m], &args.kmap, 0, row, bar, policy);
+          tma_load_2d(ring[slot].v[m], &args.vmap, 0, row, bar, policy);
+        }
+      }
+    }
+    const int mine = lane & 1 ? raw[1] : raw[0];
+    if (mine >= 0) {
+      const long long block = (long long) mine * kv.n_kv_heads + head;
+      scale[0] = kv.k_scale[block], scale[1] = kv.v_scale[block];
     }
   };
 
@@ -213,12 +242,20 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
     }
   }
   bool huge = false;
-  int  pg[2], pn[2];
-  int step = begin + warp;
-  pg[0] = page_of(step, 0), pg[1] = page_of(step, 1);
-  load_k(step, pg);
-  load_v(step, pg);
-  pn[0] = page_of(step + kWarps, 0), pn[1] = page_of(step + kWarps, 1);
+  int  step = begin + warp;
+  int   pg[kStages][2], ahead[2];  // pages of the steps in the ring, and of the one after them
+  float scale[kStages][2];         // and scales
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    ask(step + i * kWarps, pg[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    fetch(step + i * kWarps, i, pg[i], scale[i]);
+  }
+  ask(step + kStages * kWarps, ahead);
+  int      slot   = 0;
+  uint32_t parity = 0;
   __syncthreads();  // the queries are in place
   float unit[NT][2];
 #pragma unroll
@@ -229,16 +266,25 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
     }
   }
 
+#pragma unroll 1
   for (; step < end; step += kWarps) {
+    Stage &st = ring[slot];
+    if (!__all_sync(0xffffffffu, mbar_wait(&bars[warp][slot], parity))) {
+      record_error(a.err, kErrWait);
+      break;
+    }
     // ---- scores
     float s[2][NT][4];
     float by[2], up[2], inv[2];
+    block_scales(scale[0][0], scale[0][1], a.scale_log2, by[0], up[0], inv[0]);  // (of the lane's tile)
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const float v = vs[m] > 0.f ? vs[m] : 1.f;
-      by[m]         = pg[m] >= 0 && ks[m] > 0.f ? ks[m] * a.scale_log2 : a.scale_log2;
-      up[m]         = pg[m] >= 0 ? log2f(v) : 0.f;
-      inv[m]        = pg[m] >= 0 ? 1.f / v : 0.f;
+    for (int m = 1; m >= 0; --m) {
+      by[m]  = __shfl_sync(0xffffffffu, by[0], m);
+      up[m]  = __shfl_sync(0xffffffffu, up[0], m);
+      inv[m] = __shfl_sync(0xffffffffu, inv[0], m);
+      if (pg[0][m] < 0) {
+        by[m] = 1.f, up[m] = inv[m] = 0.f;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
@@ -253,15 +299,16 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int x = 0; x < TERMS; ++x) {
-            qf[n][x] = *reinterpret_cast<const uint4 *>(&sm.q[x][n * 8 + g][i * 64 + t * 16 + w2 * 8]);
+            qf[n][x] = *reinterpret_cast<const uint4 *>(&sm_q[x][n * 8 + g][i * 64 + t * 16 + w2 * 8]);
           }
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
+          const uint2 k0 = *reinterpret_cast<const uint2 *>(st.k[m] + swizzled<D>(token_of(g), 4 * i + t) + 8 * w2);
+          const uint2 k1 = *reinterpret_cast<const uint2 *>(st.k[m] + swizzled<D>(token_of(g) + 8, 4 * i + t) + 8 * w2);
 #pragma unroll
           for (int w1 = 0; w1 < 2; ++w1) {
-            const uint32_t c0 = w2 ? (w1 ? kr[m][0][i].w : kr[m][0][i].z) : (w1 ? kr[m][0][i].y : kr[m][0][i].x);
-            const uint32_t c1 = w2 ? (w1 ? kr[m][1][i].w : kr[m][1][i].z) : (w1 ? kr[m][1][i].y : kr[m][1][i].x);
+            const uint32_t c0 = w1 ? k0.y : k0.x, c1 = w1 ? k1.y : k1.x;
             uint32_t       h0[2], h1[2];
             codes_to_h2<KVT>(c0, h0);
             codes_to_h2<KVT>(c1, h1);
@@ -277,11 +324,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
         }
       }
     }
-    const bool next = step + kWarps < end;
-    const int  live[2] = { pg[0], pg[1] };
-    if (next) {
-      load_k(step + kWarps, pn);
-    }
+    const int live[2] = { pg[0][0], pg[0][1] };
     // ---- weights
     const int  tok0 = step * kStep;
     const bool full = live[0] >= 0 && live[1] >= 0 && tok0 >= all_from && tok0 + kStep - 1 <= all_to;
@@ -292,7 +335,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int tok = tok0 + m * 16 + g + (e >> 1) * 8;
+            const int tok = tok0 + m * 16 + token_of(g) + (e >> 1) * 8;
             if (live[m] < 0 || tok > last[n][e & 1] || tok < first[n][e & 1]) {
               s[m][n][e] = -INFINITY;
             }
@@ -380,24 +423,28 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       }
     }
     // ---- O^T += V^T P^T
-    // (codes behind the context may be no numbers: their weight 0 would not hide them)
-    if (!full) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
+    for (int m = 0; m < 2; ++m) {
+      uint32_t vr[4][VW];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int tok = tok0 + m * 16 + 2 * t + (r & 1) + (r >> 1) * 8;
-          if (live[m] < 0 || tok >= hi || tok < lo) {
+      for (int r = 0; r < 4; ++r) {
+        const int row = token_of(2 * t + (r & 1)) + (r >> 1) * 8;  // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+        if constexpr (VW == 4) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(st.v[m] + swizzled<D>(row, g));
+          vr[r][0] = v.x, vr[r][1] = v.y, vr[r][2] = v.z, vr[r][3] = v.w;
+        } else {
+          const uint2 v = *reinterpret_cast<const uint2 *>(st.v[m] + swizzled<D>(row, g >> 1) + (g & 1) * 8);
+          vr[r][0] = v.x, vr[r][1] = v.y;
+        }
+        // (codes behind the context may be no numbers: their weight 0 would not hide them)
+        const int tok = tok0 + m * 16 + row;
+        if (!full && (live[m] < 0 || tok >= hi || tok < lo)) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              vr[m][r][w] = 0;
-            }
+          for (int w = 0; w < VW; ++w) {
+            vr[r][w] = 0;
           }
         }
       }
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
 #pragma unroll
@@ -405,8 +452,8 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
           // codes (token A, token B) of d = 4 w + 2 half and of the one after it, side by side
           const uint32_t sel = half ? 0x7362 : 0x5140;
           uint32_t       ab[2], cd[2];
-          codes_to_h2<KVT>(__byte_perm(vr[m][0][w], vr[m][1][w], sel), ab);
-          codes_to_h2<KVT>(__byte_perm(vr[m][2][w], vr[m][3][w], sel), cd);
+          codes_to_h2<KVT>(__byte_perm(vr[0][w], vr[1][w], sel), ab);
+          codes_to_h2<KVT>(__byte_perm(vr[2][w], vr[3][w], sel), cd);
           const uint32_t af[4] = { ab[0], ab[1], cd[0], cd[1] };
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -418,15 +465,23 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
         }
       }
     }
-    if (next) {
-      load_v(step + kWarps, pn);
-      pg[0] = pn[0], pg[1] = pn[1];
-      pn[0] = page_of(step + 2 * kWarps, 0), pn[1] = page_of(step + 2 * kWarps, 1);
+    // the slot takes the step after those in the ring
+    __syncwarp();  // (everybody has used what lay there)
+#pragma unroll
+    for (int i = 0; i + 1 < kStages; ++i) {
+      pg[i][0] = pg[i + 1][0], pg[i][1] = pg[i + 1][1];
+      scale[i][0] = scale[i + 1][0], scale[i][1] = scale[i + 1][1];
+    }
+    fetch(step + kStages * kWarps, slot, ahead, scale[kStages - 1]);
+    pg[kStages - 1][0] = ahead[0], pg[kStages - 1][1] = ahead[1];
+    ask(step + (kStages + 1) * kWarps, ahead);
+    if (++slot == kStages) {
+      slot = 0, parity ^= 1;
     }
   }
 
   // ---- the warps' results, in warp order
-  __syncthreads();  // the queries are no longer needed
+  __syncthreads();  // the rings are no longer needed
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -442,7 +497,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        *reinterpret_cast<float2 *>(&sm.o[warp][c][g * (D / 8) + 2 * i]) = make_float2(o[n][i][j], o[n][i][j + 2]);
+        *reinterpret_cast<float2 *>(&sm_o[warp][c][g * (D / 8) + 2 * i]) = make_float2(o[n][i][j], o[n][i][j + 2]);
       }
     }
   }
@@ -462,7 +517,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float  f = exp2_approx(ml[w][0][c] - m);
-      const float4 v = *reinterpret_cast<const float4 *>(&sm.o[w][c][d]);
+      const float4 v = *reinterpret_cast<const float4 *>(&sm_o[w][c][d]);
       sum            = fmaf(f, ml[w][1][c], sum);
       acc[p].x = fmaf(f, v.x, acc[p].x), acc[p].y = fmaf(f, v.y, acc[p].y);
       acc[p].z = fmaf(f, v.z, acc[p].z), acc[p].w = fmaf(f, v.w, acc[p].w);
@@ -477,7 +532,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       const int i = threadIdx.x + p * kThreads, c = i / (D / 4), d = i % (D / 4) * 4;
-      *reinterpret_cast<float4 *>(&sm.o[0][c][d]) = acc[p];
+      *reinterpret_cast<float4 *>(&sm_o[0][c][d]) = acc[p];
       if (d == 0) {
         ml[0][0][c] = m_cta[p], ml[0][1][c] = l_cta[p];
       }
@@ -528,7 +583,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
     }
     for (int r = 0; r < a.splits; ++r) {
       const float  f = exp2_approx(*cluster.map_shared_rank(&ml[0][0][c], r) - m);
-      const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sm.o[0][c][d], r));
+      const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(&sm_o[0][c][d], r));
       sum            = fmaf(f, *cluster.map_shared_rank(&ml[0][1][c], r), sum);
       v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
     }
@@ -575,15 +630,43 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   }
 }
 
+// codes as rows of d bytes, fetched 16 rows at a time with 16-byte chunks swizzled over the row
+bool codes_map(CUtensorMap *map, const uint8_t *codes, long long rows, int d) {
+  using EncodeTiledFn = decltype(&cuTensorMapEncodeTiled);
+  static EncodeTiledFn enc = [] {
+    void                           *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  const cuuint64_t dim[2] = { (cuuint64_t) d, (cuuint64_t) rows }, stride[1] = { (cuuint64_t) d };
+  const cuuint32_t box[2] = { (cuuint32_t) d, 16 }, step[2] = { 1, 1 };
+  return enc && enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(codes), dim, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int KVT, int D, bool F32>
 cudaError_t launch_tiles(const AttnArgs &a, const AttnPlan &p, bool pdl, cudaStream_t st) {
   const long long grid = (long long) a.kv.n_seqs * p.col_groups * a.kv.n_kv_heads * p.groups * p.splits;
   if (grid > 0x7fffffffll) {
     return cudaErrorInvalidConfiguration;
   }
-  const cudaError_t e = p.col_tiles == 1
-                    ? launch_decoder_kernel(attn_decode_kernel<KVT, D, 1, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st)
-                    : launch_decoder_kernel(attn_decode_kernel<KVT, D, 2, F32>, a, (unsigned) grid, kThreads, 0, pdl, p.splits, st);
+  constexpr int smem = (int) sizeof(DecodeStage<D>) * kWarps * kStages + 1024;
+  DecodeArgs    args;
+  args.a               = a;
+  const long long rows = (long long) a.kv.n_pages * a.kv.n_kv_heads * a.kv.page_size;
+  if (!codes_map(&args.kmap, a.kv.k_codes, rows, D) || !codes_map(&args.vmap, a.kv.v_codes, rows, D)) {
+    return cudaErrorInvalidValue;
+  }
+  auto launch = [&](auto kernel) {
+    const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
+    return e != cudaSuccess ? e : launch_decoder_kernel(kernel, args, (unsigned) grid, kThreads, smem, pdl, p.splits, st);
+  };
+  const cudaError_t e = p.col_tiles == 1 ? launch(attn_decode_kernel<KVT, D, 1, F32>) : launch(attn_decode_kernel<KVT, D, 2, F32>);
   return e != cudaSuccess || p.groups == 1 ? e : attn_join_launch(a, D, !F32, pdl, st);
 }
 
@@ -611,7 +694,7 @@ AttnPlan attn_plan(int sm_count, int n_seqs, int n_rows, int n_kv_heads, int gro
   AttnPlan        p    = {};
   const long long cols = (long long) max_q * group;
   p.splits = p.groups = p.col_tiles = p.col_groups = 1;
-  long long jobs, want, least;  // CTAs of one pass over the contexts, CTAs wanted, tokens worth a CTA of its own
+  long long jobs;  // CTAs of one pass over the contexts
   if (cols > 32 && group <= 128) {
     p.tile              = true;
     const int per_tile  = 128 / group;
@@ -619,21 +702,42 @@ AttnPlan attn_plan(int sm_count, int n_seqs, int n_rows, int n_kv_heads, int gro
     const int per_cta   = p.two_row_tiles ? 2 * per_tile : per_tile;
     p.row_slots         = n_rows / per_cta + (long long) n_seqs;
     jobs                = ((long long) n_rows + per_cta - 1) / per_cta * n_kv_heads;
-    want = sm_count, least = 1024;
   } else {
     p.col_tiles  = cols > 8 ? 2 : 1;
     p.col_groups = (int) ((cols + 8 * p.col_tiles - 1) / (8 * p.col_tiles));
-    // enough CTAs for about four on every SM, none with less than a step per warp
-    jobs = (long long) n_seqs * n_kv_heads * p.col_groups, want = 4ll * sm_count;
-    const long long most = ((long long) max_ctx + kStep * kWarps - 1) / (kStep * kWarps);
-    while (p.splits < 8 && jobs * p.splits < want && p.splits < most) {
-      p.splits *= 2;
+    jobs         = (long long) n_seqs * n_kv_heads * p.col_groups;
+    const long long slots = (long long) sm_count * (p.col_tiles == 1 ? 3 : 2);  // CTAs resident at once
+    const long long most  = ((long long) max_ctx + kStep * kWarps - 1) / (kStep * kWarps);  // a step per warp
+    // Few short contexts: a cluster over each, joined in shared memory - one launch (700 tokens of one sequence
+    // and 8 heads: 7.3 us in clusters of 8, 9.7 us through the workspace, 12.5 us unsplit).
+    if (jobs * 8 <= slots && max_ctx <= 8192) {
+      while (p.splits < 8 && p.splits < most) {
+        p.splits *= 2;
+      }
+      return p;
     }
-    jobs *= p.splits;
-    least = p.splits == 8 ? 4096 : 1 << 30;
+    // Else independent CTAs joined by a second launch, which leave no SM waiting for a cluster's worth of room:
+    // one wave of equal shares when there are fewer jobs than CTAs fit (2 x 8 jobs of 131072 tokens: 112 us in 27
+    // shares, 138 in 32, 154 in clusters of 8), about four waves, for lengths that differ, otherwise (64 x 8
+    // jobs of 1 .. 8192 tokens: 101 us in 4 shares, 119 unsplit, 113 in 8, 110 in clusters of 2).
+    long long want_groups = jobs >= slots / 2 ? (4 * slots + jobs - 1) / jobs : slots / jobs;
+    want_groups = want_groups < max_ctx / 1024 ? want_groups : max_ctx / 1024;
+    p.groups    = want_groups < 1 ? 1 : (want_groups > 64 ? 64 : (int) want_groups);
+    if (attn_part_bytes(n_seqs, max_q, n_kv_heads * group, head_dim, p.groups) > workspace_bytes) {
+      // no room to join them: clusters, and as many shares as the room allows
+      p.groups = 1;
+      while (p.splits < 8 && jobs * p.splits < slots && p.splits < most) {
+        p.splits *= 2;
+      }
+      while (p.groups < 16 && jobs * p.splits * p.groups * 2 <= slots && max_ctx / (2 * p.groups) >= 4096 &&
+             attn_part_bytes(n_seqs, max_q, n_kv_heads * group, head_dim, 2 * p.groups) <= workspace_bytes) {
+        p.groups *= 2;
+      }
+    }
+    return p;
   }
-  // several CTAs (clusters) over one context whose results a second launch joins: when each still has enough tokens
-  while (p.groups < 16 && jobs * p.groups < want && max_ctx / (2 * p.groups) >= least) {
+  // several CTAs over one context whose results a second launch joins: when each still has enough keys
+  while (p.groups < 16 && jobs * p.groups < sm_count && max_ctx / (2 * p.groups) >= 1024) {
     p.groups *= 2;
   }
   while (p.groups > 1 && attn_part_bytes(n_seqs, max_q, n_kv_heads * group, head_dim, p.groups) > workspace_bytes) {

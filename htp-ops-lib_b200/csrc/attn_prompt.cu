@@ -624,9 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         if (p < 0 || p >= kv.n_pages) {
           record_error(a.err, kErrPage);
         } else {
-          const float ks = kv.k_scale[(long long) p * kv.n_kv_heads + head], vs = kv.v_scale[(long long) p * kv.n_kv_heads + head];
-          const float v  = vs > 0.f ? vs : 1.f;
-          by = (ks > 0.f ? ks : 1.f) * a.scale_log2, up = log2f(v), inv = 1.f / v;
+          const long long at_p = (long long) p * kv.n_kv_heads + head;
+          block_scales(kv.k_scale[at_p], kv.v_scale[at_p], a.scale_log2, by, up, inv);
         }
       }
       __syncwarp();
@@ -738,7 +737,7 @@ cudaError_t launch(const AttnArgs &a, bool pdl, cudaStream_t st) {
     return cudaErrorInvalidConfiguration;
   }
   constexpr int     smem = Sizes<D>::kSmem;
-  const cudaError_t e    = cudaFuncSetAttribute(attn_prompt_kernel<KVT, D, F32, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const cudaError_t e    = allow_smem(reinterpret_cast<const void *>(attn_prompt_kernel<KVT, D, F32, ROWS>), smem);
   return e != cudaSuccess ? e : launch_decoder_kernel(attn_prompt_kernel<KVT, D, F32, ROWS>, a, (unsigned) grid, kThreads, smem, pdl, 1, st);
 }
 

@@ -6,6 +6,8 @@
 #include <cmath>
 #include <map>
 #include <mutex>
+#include <set>
+#include <utility>
 
 #include "device_ctx.h"
 #include "htp_ops_b200.h"
@@ -51,7 +53,8 @@ bool sizes_ok(const HtpB200PagedKv *kv) {
   return kv && kv->n_pages > 0 && (kv->page_size == 16 || kv->page_size == 32 || kv->page_size == 64 || kv->page_size == 128) &&
          kv->n_kv_heads > 0 && kv->n_kv_heads <= 65536 && (kv->head_dim == 64 || kv->head_dim == 128) &&
          (kv->kv_type == HTP_B200_KV_I8 || kv->kv_type == HTP_B200_KV_E4M3) && kv->n_seqs > 0 && kv->table_stride > 0 &&
-         kv->n_rows > 0 && kv->n_rows <= kMaxLength && kv->n_seqs <= kMaxLength;
+         kv->n_rows > 0 && kv->n_rows <= kMaxLength && kv->n_seqs <= kMaxLength &&
+         (int64_t) kv->n_pages * kv->n_kv_heads <= 0x7fffffff / kv->page_size;
 }
 
 bool view_of(const HtpB200PagedKv *kv, KvView *v) {
@@ -115,6 +118,24 @@ int *device_error_word(DeviceCtx *ctx) {
   }
   *static_cast<int *>(p) = 0;
   return g_err_words[ctx->device] = static_cast<int *>(p);
+}
+
+cudaError_t allow_smem(const void *kernel, int bytes) {
+  int device = -1;
+  if (const cudaError_t e = cudaGetDevice(&device); e != cudaSuccess) {
+    return e;
+  }
+  static std::mutex                                mu;
+  static std::set<std::pair<int, const void *>>    done_for;
+  std::lock_guard<std::mutex>                      lk(mu);
+  if (done_for.count({ device, kernel })) {
+    return cudaSuccess;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) {
+    done_for.insert({ device, kernel });
+  }
+  return e;
 }
 
 int take_device_error(DeviceCtx *ctx) {

@@ -97,6 +97,9 @@ struct LogitsArgs {
 };
 cudaError_t logits_process_launch(const LogitsArgs &a, int sm_count, bool pdl, cudaStream_t stream);
 
+// Dynamic shared memory of a kernel on the current device, set once per kernel and device (decoder_ops.cu).
+cudaError_t allow_smem(const void *kernel, int bytes);
+
 // Launch with or without programmatic stream serialisation, in clusters of `cluster` CTAs.
 template <typename Kernel, typename Args>
 inline cudaError_t launch_decoder_kernel(Kernel kernel, const Args &args, unsigned grid, unsigned threads, size_t smem,
