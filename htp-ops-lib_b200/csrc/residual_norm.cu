@@ -13,6 +13,7 @@ namespace htp {
 namespace {
 
 constexpr int kMaxThreads = 1024;
+constexpr int kManyThreads = 512;
 
 __device__ __forceinline__ float cta_sum(float v, float *red) {
 #pragma unroll
@@ -23,11 +24,13 @@ __device__ __forceinline__ float cta_sum(float v, float *red) {
     red[threadIdx.x >> 5] = v;
   }
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < (int) blockDim.x / 32; ++i) {
-    s += red[i];
+  const int lane = threadIdx.x & 31;
+  v              = lane < (int) blockDim.x / 32 ? red[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, o);
   }
-  return s;
+  return v;
 }
 
 template <int W>
@@ -37,6 +40,16 @@ __device__ __forceinline__ void ld(const float *p, float (&x)[W]) {
     x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
   } else {
     x[0] = *p;
+  }
+}
+// read once: not kept
+template <int W>
+__device__ __forceinline__ void ld_row(const float *p, float (&x)[W]) {
+  if constexpr (W == 4) {
+    const float4 v = __ldcs(reinterpret_cast<const float4 *>(p));
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    x[0] = __ldcs(p);
   }
 }
 template <int W>
@@ -96,20 +109,31 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(const __grid_
     }
   };
   if constexpr (V > 0) {
-    float h[V][W], bv[V][W];
-    float ss = 0.f;
+    // every operand is asked for before the first sum waits for its row (the longest rows leave no registers for
+    // that: gate and weights are read where they are used)
+    constexpr bool EARLY = V <= 2;
+    float h[V][W], bv[V][W], pw[V][W], g[V][W], w[V][W];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int i = threadIdx.x * W + v * step;
       if (i < a.n) {
-        ld<W>(x + i, h[v]);
+        ld_row<W>(x + i, h[v]);
         if (block) {
-          ld<W>(block + i, bv[v]);
+          ld_row<W>(block + i, bv[v]);
+        }
+        if (EARLY && gate) {
+          ld<W>(gate + i, g[v]);
+        }
+        if (EARLY && a.post_weight) {
+          ld<W>(a.post_weight + i, pw[v]);
+        }
+        if (EARLY && a.weight) {
+          ld<W>(a.weight + i, w[v]);
         }
       }
     }
-    float post = 1.f;
-    if (block && a.post_weight) {
+    float ss = 0.f, post = 1.f;
+    if (a.post_weight) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (threadIdx.x * W + v * step < a.n) {
@@ -126,15 +150,24 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(const __grid_
     for (int v = 0; v < V; ++v) {
       const int i = threadIdx.x * W + v * step;
       if (i < a.n) {
-        if (block) {
-          residual(i, post, h[v], bv[v]);
+        if (!EARLY && gate) {
+          ld<W>(gate + i, g[v]);
         }
-        if (h_out) {
-          st<W>(h_out + i, h[v]);
+        if (!EARLY && a.post_weight) {
+          ld<W>(a.post_weight + i, pw[v]);
         }
 #pragma unroll
         for (int e = 0; e < W; ++e) {
+          if (block) {
+            float b = bv[v][e];
+            b       = a.post_weight ? b * post * pw[v][e] : b;
+            b       = gate ? b * g[v][e] : b;
+            h[v][e] = fmaf(a.block_scale, b, h[v][e]);
+          }
           ss = fmaf(h[v][e], h[v][e], ss);
+        }
+        if (h_out) {
+          st<W>(h_out + i, h[v]);
         }
       }
     }
@@ -146,13 +179,12 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(const __grid_
     for (int v = 0; v < V; ++v) {
       const int i = threadIdx.x * W + v * step;
       if (i < a.n) {
-        float w[W];
-        if (a.weight) {
-          ld<W>(a.weight + i, w);
+        if (!EARLY && a.weight) {
+          ld<W>(a.weight + i, w[v]);
         }
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          h[v][e] = a.weight ? h[v][e] * scale * w[e] : h[v][e] * scale;
+          h[v][e] = a.weight ? h[v][e] * scale * w[v][e] : h[v][e] * scale;
         }
         st<W>(out + i, h[v]);
       }
@@ -216,8 +248,11 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(const __grid_
 template <int W, typename Out>
 cudaError_t launch_width(const AddRmsNormArgs &a, bool pdl, cudaStream_t st) {
   const long long groups  = ((long long) a.n + W - 1) / W;
+  // Few rows: as many threads as there are groups, for the latency.  Many: fewer threads with more groups each, so
+  // that more rows are on an SM at once.
+  const int       most    = a.rows > 296 ? kManyThreads : kMaxThreads;
   const long long t1      = (groups + 31) / 32 * 32;
-  const unsigned  threads = (unsigned) (t1 < kMaxThreads ? t1 : kMaxThreads);
+  const unsigned  threads = (unsigned) (t1 < most ? t1 : (groups > 4ll * most ? kMaxThreads : most));
   const long long per     = (groups + threads - 1) / threads;
   const unsigned  grid    = (unsigned) a.rows;
   if (per <= 1) {
