@@ -27,6 +27,11 @@ HTP_OPS_FLASH_ATTN_QO_F32_KV_F16 = 5
 HTP_OPS_MAT_MUL_W4D16A16 = 6
 HTP_OPS_MAT_MUL_W8D16A16 = 7
 HTP_OPS_COUNT = 8
+# enum HtpOpsDecoderIndex: the operators around a decoder's matmuls
+HTP_OPS_KV_APPEND = 16
+HTP_OPS_ATTN_PAGED = 17
+HTP_OPS_ADD_RMS_NORM = 18
+HTP_OPS_LOGITS_PROCESS = 19
 
 # enum RequestType (include/message.h)
 REQUEST_TYPE_NO_OP = 0
@@ -167,6 +172,61 @@ def pack_rms_norm_request(dst: tuple[int, int], src: tuple[int, int], ne0: int, 
     """RequestHeader{state=0,type=OP_COMPUTE} || OpComputeRequest{RMS_NORM_F32} || RmsNormF32Params - 36 bytes."""
     return struct.pack("<iiI6i", 0, REQUEST_TYPE_OP_COMPUTE, HTP_OPS_RMS_NORM_F32, dst[0], dst[1], src[0], src[1], ne0,
                        ne1)
+
+
+_ABSENT = (0, 0)  # a buffer that the request does not have
+
+
+def _pack_decoder_request(op: int, fmt: str, *values) -> bytes:
+    return struct.pack("<iiI" + fmt, 0, REQUEST_TYPE_OP_COMPUTE, op, *values)
+
+
+def _buffers(*addresses) -> list[int]:
+    return [v for a in addresses for v in (a or _ABSENT)]
+
+
+def _paged_kv(kv: dict) -> list[int]:
+    """struct PagedKvParams: `kv` has the fields of PagedKv, its buffers as (handle, offset)."""
+    names = [n for n, _ in PagedKv._fields_]
+    return _buffers(*(kv[n] for n in names[:7])) + [kv[n] for n in names[7:]]
+
+
+def pack_kv_append_request(kv: dict, k, v, k_stride: int, v_stride: int, act_type: int, q=None, q_out=None,
+                           q_stride: int = 0, q_out_stride: int = 0, n_heads: int = 0, q_out_type: int = ACT_F32,
+                           rope_table=None, positions=None, rope_mode: int = ROPE_NONE, rot_dim: int = 0,
+                           table_len: int = 0) -> bytes:
+    """RequestHeader || OpComputeRequest{KV_APPEND} || KvAppendParams; buffers are (handle, offset) or None."""
+    return _pack_decoder_request(HTP_OPS_KV_APPEND, "44i", *_paged_kv(kv),
+                                 *_buffers(k, v, q, q_out, rope_table, positions), k_stride, v_stride, q_stride,
+                                 q_out_stride, n_heads, act_type, q_out_type, rope_mode, rot_dim, table_len)
+
+
+def pack_attn_paged_request(kv: dict, out, q, out_stride: int, q_stride: int, n_heads: int, act_type: int, scale: float,
+                            window: int, max_q: int, max_ctx: int, workspace=None, workspace_bytes: int = 0) -> bytes:
+    """RequestHeader || OpComputeRequest{ATTN_PAGED} || AttnPagedParams."""
+    return _pack_decoder_request(HTP_OPS_ATTN_PAGED, "33if3i", *_paged_kv(kv), *_buffers(out, q, workspace),
+                                 workspace_bytes, out_stride, q_stride, n_heads, act_type, scale, window, max_q,
+                                 max_ctx)
+
+
+def pack_add_rms_norm_request(x, n: int, rows: int, h_out=None, norm_out=None, block=None, post_weight=None, gate=None,
+                              gate_stride: int = 0, weight=None, block_scale: float = 1.0, eps: float = 1e-5,
+                              norm_type: int = ACT_F32) -> bytes:
+    """RequestHeader || OpComputeRequest{ADD_RMS_NORM} || AddRmsNormParams."""
+    return _pack_decoder_request(HTP_OPS_ADD_RMS_NORM, "15i2f3i",
+                                 *_buffers(h_out, norm_out, x, block, post_weight, gate, weight), gate_stride,
+                                 block_scale, eps, n, rows, norm_type)
+
+
+def pack_logits_process_request(dst, src, stride: int, rows: int, vocab: int, n_history: int = 0, n_bias: int = 0,
+                                n_mask_rows: int = 0, **buffers) -> bytes:
+    """RequestHeader || OpComputeRequest{LOGITS_PROCESS} || LogitsProcessParams; `buffers` by the names of LogitsParams."""
+    names = [n for n, _ in LogitsParams._fields_][:11]
+    unknown = set(buffers) - set(names)
+    if unknown:
+        raise TypeError(f"no such buffers: {sorted(unknown)}")
+    return _pack_decoder_request(HTP_OPS_LOGITS_PROCESS, "32i", *_buffers(dst, src, *(buffers.get(n) for n in names)),
+                                 stride, rows, vocab, n_history, n_bias, n_mask_rows)
 
 
 def pack_map_request(puts: list[int], gets: list[int] | None = None) -> bytes:

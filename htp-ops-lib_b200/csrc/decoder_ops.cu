@@ -298,7 +298,7 @@ int htp_b200_logits_process(float *dst, const float *src, int64_t stride, int ro
     return -1;
   }
   if ((p->history && p->n_history < 0) || (p->bias_token && p->n_bias < 0) || (p->mask && p->n_mask_rows <= 0) ||
-      (p->mask_row && !p->mask)) {
+      (p->mask_row && !p->mask) || (p->mask && !p->mask_row && p->n_mask_rows < rows)) {
     return -1;
   }
   const void *ints[] = { p->history, p->history_start, p->prompt_len, p->repetition, p->presence, p->frequency,

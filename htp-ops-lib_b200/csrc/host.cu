@@ -16,6 +16,7 @@
 #include <mutex>
 #include <thread>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "device_ctx.h"
@@ -189,6 +190,147 @@ int flush_batch() {
   return rc;
 }
 
+// Bytes of the parameter block of an operator.
+size_t params_size(uint32_t op) {
+  switch (op) {
+    case HTP_OPS_RMS_NORM_F32: return sizeof(RmsNormF32Params);
+    case HTP_OPS_KV_APPEND: return sizeof(KvAppendParams);
+    case HTP_OPS_ATTN_PAGED: return sizeof(AttnPagedParams);
+    case HTP_OPS_ADD_RMS_NORM: return sizeof(AddRmsNormParams);
+    case HTP_OPS_LOGITS_PROCESS: return sizeof(LogitsProcessParams);
+    default: return sizeof(MatMulParams);
+  }
+}
+
+// Handles -> addresses of one request's buffers.  An absent one (fd <= 0) is nullptr; a region that is no part
+// of its buffer, or of no size, makes the request fail.
+struct Regions {
+  bool ok = true;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+
+  template <typename T = void>
+  T *at(const RpcmemBufAddr &a, int64_t bytes, bool writes = false) {
+    if (a.fd <= 0) {
+      return nullptr;
+    }
+    uint8_t *p = bytes > 0 ? resolve(a, (size_t) bytes) : nullptr;
+    ok         = ok && p;
+    if (p && writes) {
+      written.emplace_back((uintptr_t) p, (uintptr_t) p + (size_t) bytes);
+    }
+    return reinterpret_cast<T *>(p);
+  }
+};
+
+// bytes of `rows` rows of `width` elements, `stride` apart; 0 where the numbers make no sense
+int64_t rows_bytes(int64_t rows, int64_t stride, int64_t width, int act_type) {
+  constexpr int64_t kMost = 1 << 30;  // (no product below leaves 64 bits)
+  return rows > 0 && rows <= kMost && width > 0 && stride >= width && stride <= kMost ? ((rows - 1) * stride + width) * (act_type == HTP_B200_ACT_F16 ? 2 : 4) : 0;
+}
+
+HtpB200PagedKv paged_kv(const PagedKvParams &p, bool writes, Regions &r) {
+  HtpB200PagedKv kv = {};
+  if (p.n_pages <= 0 || p.page_size <= 0 || p.page_size > 128 || p.n_kv_heads <= 0 || p.n_kv_heads > 65536 || p.head_dim <= 0 ||
+      p.head_dim > 128 || p.n_seqs <= 0 || p.n_seqs > 1 << 30 || p.table_stride <= 0 || p.table_stride > 1 << 30) {
+    r.ok = false;
+    return kv;
+  }
+  const int64_t blocks = (int64_t) p.n_pages * p.n_kv_heads, codes = blocks * p.page_size * p.head_dim;
+  kv.k_codes    = r.at(p.k_codes, codes, writes);
+  kv.v_codes    = r.at(p.v_codes, codes, writes);
+  kv.k_scale    = r.at<float>(p.k_scale, blocks * 4, writes);
+  kv.v_scale    = r.at<float>(p.v_scale, blocks * 4, writes);
+  kv.page_table = r.at<int32_t>(p.page_table, (int64_t) p.n_seqs * p.table_stride * 4);
+  kv.q_start    = r.at<int32_t>(p.q_start, ((int64_t) p.n_seqs + 1) * 4);
+  kv.ctx_len    = r.at<int32_t>(p.ctx_len, (int64_t) p.n_seqs * 4);
+  kv.n_pages = p.n_pages, kv.page_size = p.page_size, kv.n_kv_heads = p.n_kv_heads, kv.head_dim = p.head_dim;
+  kv.kv_type = p.kv_type, kv.n_seqs = p.n_seqs, kv.table_stride = p.table_stride, kv.n_rows = p.n_rows;
+  return kv;
+}
+
+// The operators around the matmuls: same functions as the raw entry points, on the session stream, behind
+// whatever the message has collected so far.
+int enqueue_decoder_op(uint32_t op, const uint8_t *payload) {
+  Regions r;
+  int     rc = -1;
+  if (!g.batch.ops.empty()) {
+    flush_batch();  // stream order then covers every dependence on the pending mat-vecs
+  }
+  if (op == HTP_OPS_KV_APPEND) {
+    KvAppendParams p;
+    memcpy(&p, payload, sizeof(p));
+    const HtpB200PagedKv kv   = paged_kv(p.kv, true, r);
+    const int64_t        wide = (int64_t) kv.n_kv_heads * kv.head_dim, q_wide = (int64_t) p.n_heads * kv.head_dim;
+    HtpB200Rope          rope = {};
+    rope.table_len = p.table_len, rope.rot_dim = p.rot_dim, rope.mode = p.rope_mode;
+    if (p.rope_mode != HTP_B200_ROPE_NONE) {
+      rope.table     = r.at<float>(p.rope_table, rows_bytes(p.table_len, p.rot_dim, p.rot_dim, HTP_B200_ACT_F32));
+      rope.positions = r.at<int32_t>(p.positions, (int64_t) kv.n_rows * 4);
+    }
+    const void *k = r.at(p.k, rows_bytes(kv.n_rows, p.k_stride, wide, p.act_type));
+    const void *v = r.at(p.v, rows_bytes(kv.n_rows, p.v_stride, wide, p.act_type));
+    const void *q = r.at(p.q, rows_bytes(kv.n_rows, p.q_stride, q_wide, p.act_type));
+    void       *o = q ? r.at(p.q_out, rows_bytes(kv.n_rows, p.q_out_stride, q_wide, p.q_out_type), true) : nullptr;
+    if (r.ok) {
+      rc = htp_b200_kv_append(&kv, &rope, k, p.k_stride, v, p.v_stride, q, p.q_stride, o, p.q_out_stride, p.n_heads, p.act_type,
+                              p.q_out_type, g.stream);
+    }
+  } else if (op == HTP_OPS_ATTN_PAGED) {
+    AttnPagedParams p;
+    memcpy(&p, payload, sizeof(p));
+    const HtpB200PagedKv kv   = paged_kv(p.kv, false, r);
+    const int64_t        wide = (int64_t) p.n_heads * kv.head_dim;
+    void       *out = r.at(p.out, rows_bytes(kv.n_rows, p.out_stride, wide, p.act_type), true);
+    const void *q   = r.at(p.q, rows_bytes(kv.n_rows, p.q_stride, wide, p.act_type));
+    void       *ws  = p.workspace_bytes > 0 ? r.at(p.workspace, p.workspace_bytes, true) : nullptr;
+    if (r.ok) {
+      rc = htp_b200_attn_paged(out, p.out_stride, q, p.q_stride, &kv, p.n_heads, p.act_type, p.scale, p.window, p.max_q, p.max_ctx, ws,
+                               ws ? (size_t) p.workspace_bytes : 0, g.stream);
+    }
+  } else if (op == HTP_OPS_ADD_RMS_NORM) {
+    AddRmsNormParams p;
+    memcpy(&p, payload, sizeof(p));
+    const int64_t all = rows_bytes(p.rows, p.n, p.n, HTP_B200_ACT_F32), row = (int64_t) p.n * 4;
+    float       *h     = r.at<float>(p.h_out, all, true);
+    void        *norm  = r.at(p.norm_out, rows_bytes(p.rows, p.n, p.n, p.norm_type), true);
+    const float *x     = r.at<float>(p.x, all), *block = r.at<float>(p.block, all);
+    const float *post  = r.at<float>(p.post_weight, row), *weight = r.at<float>(p.weight, row);
+    const float *gate  = r.at<float>(p.gate, p.gate_stride ? rows_bytes(p.rows, p.gate_stride, p.n, HTP_B200_ACT_F32) : row);
+    if (r.ok) {
+      rc = htp_b200_add_rms_norm(h, norm, x, block, post, gate, p.gate_stride, weight, p.block_scale, p.eps, p.n, p.rows, p.norm_type, g.stream);
+    }
+  } else {
+    LogitsProcessParams p;
+    memcpy(&p, payload, sizeof(p));
+    const int64_t all = rows_bytes(p.rows, p.stride, p.vocab, HTP_B200_ACT_F32), rows = (int64_t) p.rows * 4;
+    float       *dst = r.at<float>(p.dst, all, true);
+    const float *src = r.at<float>(p.src, all);
+    HtpB200LogitsParams l = {};
+    // (a history or a list of biases of no tokens may stand in a buffer of any size)
+    l.history       = r.at<int32_t>(p.history, p.n_history > 0 ? (int64_t) p.n_history * 4 : 4);
+    l.history_start = r.at<int32_t>(p.history_start, rows + 4);
+    l.prompt_len    = r.at<int32_t>(p.prompt_len, rows);
+    l.repetition    = r.at<float>(p.repetition, rows);
+    l.presence      = r.at<float>(p.presence, rows);
+    l.frequency     = r.at<float>(p.frequency, rows);
+    l.bias_token    = r.at<int32_t>(p.bias_token, p.n_bias > 0 ? (int64_t) p.n_bias * 4 : 4);
+    l.bias_value    = r.at<float>(p.bias_value, p.n_bias > 0 ? (int64_t) p.n_bias * 4 : 4);
+    l.bias_start    = r.at<int32_t>(p.bias_start, rows + 4);
+    l.mask          = r.at<uint32_t>(p.mask, (int64_t) p.n_mask_rows * ((p.vocab + 31ll) / 32) * 4);
+    l.mask_row      = r.at<int32_t>(p.mask_row, rows);
+    l.n_history = p.n_history, l.n_bias = p.n_bias, l.n_mask_rows = p.n_mask_rows;
+    if (r.ok) {
+      rc = htp_b200_logits_process(dst, src, p.stride, p.rows, p.vocab, &l, g.stream);
+    }
+  }
+  if (rc == 0) {
+    for (const auto &w : r.written) {
+      g.pending_out.add(w.first, w.second);
+    }
+  }
+  return rc;
+}
+
 // Enqueue one operator on the session stream.  Returns the synchronous part of the result
 // (argument validation); launch and kernel-side errors surface later (flush / stream wait).
 // `owner` is the request to blame if the batch the operator joins fails to launch.
@@ -220,6 +362,9 @@ int enqueue_op(const OpComputeRequest *req, RequestHeader *owner) {
       g.pending_out.add((uintptr_t) dst, (uintptr_t) dst + bytes);
     }
     return rc;
+  }
+  if (op >= HTP_OPS_KV_APPEND && op <= HTP_OPS_LOGITS_PROCESS) {
+    return enqueue_decoder_op(op, req->payload);
   }
   int weight_type, act_type;
   switch (op) {
@@ -362,7 +507,7 @@ void servicer_loop() {
             if (rsize >= need) {
               uint32_t op;
               memcpy(&op, reinterpret_cast<const uint8_t *>(rh) + sizeof(RequestHeader), sizeof(op));
-              need += op == HTP_OPS_RMS_NORM_F32 ? sizeof(RmsNormF32Params) : sizeof(MatMulParams);
+              need += params_size(op);
             }
             if (rsize < need) {
               rh->state = -1;

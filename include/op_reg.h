@@ -16,7 +16,8 @@
  * (src/dsp/ops/mat_mul.c:572-640); with the library option "permuted_weights" indices 2, 3, 4 read the
  * reference-private permuted super-blocks instead.  Index 1 reads fp16 weights in the reference's
  * 32 x 32 tile order (src/host/test.c:303-313).  Index 0 is RMSNorm.  Index 5 (FlashAttention) is
- * not built: the dispatcher answers -1.
+ * not built: the dispatcher answers -1; attention over this library's own 8-bit cache is index 17, among the
+ * operators around a decoder's matmuls that enum HtpOpsDecoderIndex names.
  */
 #ifndef HTP_OPS_OP_REG_H
 #define HTP_OPS_OP_REG_H
@@ -37,6 +38,15 @@ enum HtpOpsIndex {
 };
 
 #define HTP_OPS_REFERENCE_COUNT 6
+
+/* The operators around a decoder's matmuls (htp_ops_b200.h says what they compute), from 16 on: the indices in
+ * between stay free for the registry above. */
+enum HtpOpsDecoderIndex {
+  HTP_OPS_KV_APPEND      = 16,
+  HTP_OPS_ATTN_PAGED     = 17,
+  HTP_OPS_ADD_RMS_NORM   = 18,
+  HTP_OPS_LOGITS_PROCESS = 19,
+};
 
 #define HTP_OPS_PACKED __attribute__((packed))
 
@@ -77,12 +87,59 @@ struct FlashAttnParams {
   int32_t head_dim;
 } HTP_OPS_PACKED;
 
+/* ---- operators 16 .. 19: the arguments of the functions in htp_ops_b200.h, buffers by handle.  A buffer with
+ * fd <= 0 is absent (NULL there).  Strides count elements. ---- */
+struct PagedKvParams {
+  struct RpcmemBufAddr k_codes, v_codes, k_scale, v_scale, page_table, q_start, ctx_len;
+  int32_t              n_pages, page_size, n_kv_heads, head_dim, kv_type, n_seqs, table_stride, n_rows;
+} HTP_OPS_PACKED;
+
+struct KvAppendParams {
+  struct PagedKvParams kv;
+  struct RpcmemBufAddr k, v, q, q_out, rope_table, positions;
+  int32_t              k_stride, v_stride, q_stride, q_out_stride;
+  int32_t              n_heads, act_type, q_out_type;
+  int32_t              rope_mode, rot_dim, table_len;
+} HTP_OPS_PACKED;
+
+struct AttnPagedParams {
+  struct PagedKvParams kv;
+  struct RpcmemBufAddr out, q, workspace;
+  int32_t              workspace_bytes;
+  int32_t              out_stride, q_stride;
+  int32_t              n_heads, act_type;
+  float                scale;
+  int32_t              window, max_q, max_ctx;
+} HTP_OPS_PACKED;
+
+struct AddRmsNormParams {
+  struct RpcmemBufAddr h_out, norm_out, x, block, post_weight, gate, weight;
+  int32_t              gate_stride;
+  float                block_scale, eps;
+  int32_t              n, rows, norm_type;
+} HTP_OPS_PACKED;
+
+struct LogitsProcessParams {
+  struct RpcmemBufAddr dst, src;
+  struct RpcmemBufAddr history, history_start, prompt_len, repetition, presence, frequency;
+  struct RpcmemBufAddr bias_token, bias_value, bias_start, mask, mask_row;
+  int32_t              stride, rows, vocab, n_history, n_bias, n_mask_rows;
+} HTP_OPS_PACKED;
+
 #if defined(__cplusplus)
+static_assert(sizeof(struct PagedKvParams) == 88 && sizeof(struct KvAppendParams) == 176 &&
+                sizeof(struct AttnPagedParams) == 148 && sizeof(struct AddRmsNormParams) == 80 &&
+                sizeof(struct LogitsProcessParams) == 128,
+              "wire size");
 static_assert(sizeof(struct RpcmemBufAddr) == 8, "wire size");
 static_assert(sizeof(struct RmsNormF32Params) == 24, "wire size");
 static_assert(sizeof(struct MatMulParams) == 36, "wire size");
 static_assert(sizeof(struct FlashAttnParams) == 60, "wire size");
 #else
+_Static_assert(sizeof(struct PagedKvParams) == 88 && sizeof(struct KvAppendParams) == 176 &&
+                 sizeof(struct AttnPagedParams) == 148 && sizeof(struct AddRmsNormParams) == 80 &&
+                 sizeof(struct LogitsProcessParams) == 128,
+               "wire size");
 _Static_assert(sizeof(struct RpcmemBufAddr) == 8, "wire size");
 _Static_assert(sizeof(struct RmsNormF32Params) == 24, "wire size");
 _Static_assert(sizeof(struct MatMulParams) == 36, "wire size");

@@ -91,7 +91,7 @@ GOOD = dict(history=A, history_start=2 * A, prompt_len=3 * A, repetition=4 * A, 
 
 
 @pytest.mark.parametrize("change", [dict(history=None), dict(history_start=None), dict(history=None, history_start=None), dict(bias_token=None), dict(bias_value=None),
-                                    dict(bias_start=None), dict(mask=None), dict(n_mask_rows=0), dict(n_history=-1), dict(n_bias=-1), dict(mask=A + 2), dict(repetition=A + 1)], ids=str)
+                                    dict(bias_start=None), dict(mask=None), dict(n_mask_rows=0), dict(mask_row=None), dict(n_history=-1), dict(n_bias=-1), dict(mask=A + 2), dict(repetition=A + 1)], ids=str)
 def test_bad_logits_parameters(pkg, lib, change):
     p = ctypes.byref(pkg.LogitsParams(**{**GOOD, **change}))
     assert lib.htp_b200_logits_process(12 * A, 13 * A, 100, 2, 100, p, None) == -1
