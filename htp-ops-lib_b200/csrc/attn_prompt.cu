@@ -47,6 +47,8 @@ struct Bars {
   float    by[kScaleRing][8], up[kScaleRing][8], inv[kScaleRing][8];  // of the tile's 16-key blocks
   float    unit[128];     // fp32 queries: the power of two that a row was divided by
   float    ml[2][2][128];  // KEYS: maximum and denominator of each stream's rows
+  // element offsets of the tiles' rows in the queries and in the output, -1 for rows that are nobody's
+  long long q_at[256], out_at[256];
 };
 
 template <int D>
@@ -155,6 +157,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     bar->abort_flag = 0;
     mbar_fence_init();
   }
+  if (threadIdx.x < (ROWS ? 256 : 128)) {
+    const int       r = threadIdx.x & 127, q = i0 + (int) (threadIdx.x >> 7) * per_tile + r / a.group;
+    const bool      in = r < per_tile * a.group && q < i1;
+    const long long h  = (long long) (head * a.group + r % a.group) * D;
+    bar->q_at[threadIdx.x]   = in ? (q0 + (long long) q) * a.q_stride + h : -1;
+    bar->out_at[threadIdx.x] = in ? (q0 + (long long) q) * a.out_stride + h : -1;
+  }
   if (warp == kMmaWarp) {
     tmem_alloc<false>(&bar->tmem, 512);
     tmem_relinquish<false>();
@@ -180,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
     const int x = warp >> 2, row = (warp & 3) * 32 + lane;
     // queries -> shared memory: 128 rows of one or two parts, a batch of loads in flight
     constexpr int CH    = D / 8;  // 16-byte chunks of a row
-    constexpr int ITEMS = (ROWS ? 2 : 1) * 128 * CH / (kSoftWarps * 32), BATCH = F32 ? 4 : 8;
+    constexpr int ITEMS = (ROWS ? 2 : 1) * 128 * CH / (kSoftWarps * 32), BATCH = F32 ? 4 : 16;
     static_assert(ITEMS % 4 == 0, "whole batches");
 #pragma unroll
     for (int i0_ = 0; i0_ < ITEMS; i0_ += BATCH < ITEMS ? BATCH : ITEMS) {
@@ -188,11 +197,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       uint4         v[NB][F32 ? 2 : 1];
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        const int  it = threadIdx.x + (i0_ + i) * kSoftWarps * 32, part = it / (128 * CH), r = it / CH % 128, c = it % CH;
-        const int  q  = i0 + part * per_tile + r / a.group;
-        const bool in = r < per_tile * a.group && q < i1;
-        const uint4 *from = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.q) +
-                            ((long long) (q0 + q) * a.q_stride + (head * a.group + r % a.group) * D + c * 8) * (F32 ? 4 : 2));
+        const int       it = threadIdx.x + (i0_ + i) * kSoftWarps * 32, c = it % CH;
+        const long long at = bar->q_at[it / CH];
+        const bool      in = at >= 0;
+        const uint4    *from = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.q) + (at + c * 8) * (F32 ? 4 : 2));
 #pragma unroll
         for (int u = 0; u < (F32 ? 2 : 1); ++u) {
           v[i][u] = make_uint4(0, 0, 0, 0);
@@ -488,11 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         constexpr int CPR = ROWB / 16;  // chunks of a row
 #pragma unroll
         for (int k = 0; k < CPR; ++k) {
-          const int i = k * 32 + lane, r = i / CPR, chunk = i % CPR, gr = (warp & 3) * 32 + r;
-          const int q = i0 + (ROWS ? x * per_tile : 0) + gr / a.group;
-          if (gr < per_tile * a.group && q < i1) {
+          const int       i = k * 32 + lane, r = i / CPR, chunk = i % CPR;
+          const long long at_o = bar->out_at[(ROWS ? warp : warp & 3) * 32 + r];
+          if (at_o >= 0) {
             const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * ROWB + ((chunk ^ (r & SWZ)) << 4));
-            const long long at_o = (long long) (q0 + q) * a.out_stride + (head * a.group + gr % a.group) * D;
             *reinterpret_cast<uint4 *>(static_cast<uint8_t *>(a.out) + at_o * (F32 ? 4 : 2) + (ROWS ? 0 : x * ROWB) + chunk * 16) = u;
           }
         }

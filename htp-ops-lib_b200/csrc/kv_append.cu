@@ -218,12 +218,29 @@ __device__ __forceinline__ void append_page(const KvAppendArgs &a, int b, int pa
 
 template <int D, bool A16, bool O16>
 __device__ __forceinline__ void rotate_row(const KvAppendArgs &a, int row) {
-  constexpr int PARTS = D / 8;
+  constexpr int PARTS = D / 8, BATCH = 2;
   const KvView &kv    = a.kv;
-  int           pos   = 0;
+  const uint8_t *src  = static_cast<const uint8_t *>(a.q) + row * a.q_stride * (A16 ? 2 : 4);
+  uint8_t       *dst  = static_cast<uint8_t *>(a.q_out) + row * a.q_out_stride * (O16 ? 2 : 4);
+  const int      items = a.n_heads * PARTS;
+  float          x[BATCH][8];
+  auto           load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * kThreads;
+      if (i < items) {
+        int lo, hi;
+        part_dims(i % PARTS, a.mode, a.rot_dim, lo, hi);
+        load4<A16>(src, i / PARTS * D + lo, x[k]);
+        load4<A16>(src, i / PARTS * D + hi, x[k] + 4);
+      }
+    }
+  };
+  load(threadIdx.x);  // (on its way while the row's position is looked up)
   if (row >= kv.q_start[kv.n_seqs]) {
     return;  // behind the last sequence
   }
+  int pos = 0;
   if (a.mode) {
     if (a.positions) {
       pos = a.positions[row];
@@ -245,33 +262,36 @@ __device__ __forceinline__ void rotate_row(const KvAppendArgs &a, int row) {
       return;
     }
   }
-  const float   *table = a.rope_table + (long long) pos * a.rot_dim;
-  const uint8_t *src   = static_cast<const uint8_t *>(a.q) + row * a.q_stride * (A16 ? 2 : 4);
-  uint8_t       *dst   = static_cast<uint8_t *>(a.q_out) + row * a.q_out_stride * (O16 ? 2 : 4);
-  for (int i = threadIdx.x; i < a.n_heads * PARTS; i += kThreads) {
-    const int head = i / PARTS, j = i % PARTS;
-    int       lo, hi;
-    part_dims(j, a.mode, a.rot_dim, lo, hi);
-    float x[8];
-    load4<A16>(src, head * D + lo, x);
-    load4<A16>(src, head * D + hi, x + 4);
-    if (a.mode) {
-      rotate8(x, table, j, a.mode, a.rot_dim);
-    }
+  const float *table = a.rope_table + (long long) pos * a.rot_dim;
+  for (int i0 = threadIdx.x; i0 < items; i0 += BATCH * kThreads) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int    at = head * D + (h ? hi : lo);
-      const float *y  = x + 4 * h;
-      if constexpr (O16) {
-        const __half2 u = __floats2half2_rn(y[0], y[1]), w = __floats2half2_rn(y[2], y[3]);
-        uint2         o;
-        o.x = *reinterpret_cast<const uint32_t *>(&u);
-        o.y = *reinterpret_cast<const uint32_t *>(&w);
-        *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(dst) + at) = o;
-      } else {
-        *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + at) = make_float4(y[0], y[1], y[2], y[3]);
+    for (int k = 0; k < BATCH; ++k) {
+      const int i = i0 + k * kThreads;
+      if (i >= items) {
+        continue;
+      }
+      const int head = i / PARTS, j = i % PARTS;
+      int       lo, hi;
+      part_dims(j, a.mode, a.rot_dim, lo, hi);
+      if (a.mode) {
+        rotate8(x[k], table, j, a.mode, a.rot_dim);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int    at = head * D + (h ? hi : lo);
+        const float *y  = x[k] + 4 * h;
+        if constexpr (O16) {
+          const __half2 u = __floats2half2_rn(y[0], y[1]), w = __floats2half2_rn(y[2], y[3]);
+          uint2         o;
+          o.x = *reinterpret_cast<const uint32_t *>(&u);
+          o.y = *reinterpret_cast<const uint32_t *>(&w);
+          *reinterpret_cast<uint2 *>(reinterpret_cast<__half *>(dst) + at) = o;
+        } else {
+          *reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + at) = make_float4(y[0], y[1], y[2], y[3]);
+        }
       }
     }
+    load(i0 + BATCH * kThreads);
   }
 }
 
