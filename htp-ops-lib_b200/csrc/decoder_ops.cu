@@ -158,8 +158,18 @@ int htp_b200_kv_append(const struct HtpB200PagedKv *kv, const struct HtpB200Rope
     return -1;
   }
   const int64_t wide = (int64_t) kv->n_kv_heads * kv->head_dim;
+  const size_t  n_scale = (size_t) kv->n_pages * kv->n_kv_heads * sizeof(float);
+  if (overlap(kv->k_codes, codes_bytes(kv), kv->v_codes, codes_bytes(kv)) || overlap(kv->k_scale, n_scale, kv->v_scale, n_scale)) {
+    return -1;  // keys and values are written by different CTAs
+  }
   if (!rows_ok(k, k_stride, wide, act_type) || !rows_ok(v, v_stride, wide, act_type)) {
     return -1;
+  }
+  for (const void *codes : { kv->k_codes, kv->v_codes }) {
+    if (overlap(k, extent(kv->n_rows, k_stride, wide, act_size(act_type)), codes, codes_bytes(kv)) ||
+        overlap(v, extent(kv->n_rows, v_stride, wide, act_size(act_type)), codes, codes_bytes(kv))) {
+      return -1;
+    }
   }
   if (q) {
     const int64_t q_wide = (int64_t) n_heads * kv->head_dim;

@@ -13,7 +13,7 @@ constexpr int kErrSequence = 302;
 constexpr int kErrPosition = 303;
 constexpr int kErrRange    = 304;
 constexpr int kErrMaskRow  = 305;
-constexpr int kErrWait     = 311;  // a bounded wait inside the prompt attention ran out
+constexpr int kErrWait     = 311;  // a bounded wait inside attention ran out
 
 constexpr float kKvMinScale = 0x1p-100f;  // scale of a block of zeros
 

@@ -245,6 +245,7 @@ struct HtpB200Rope {
  * codes of older tokens follow a grown scale: c becomes round(c * (old scale / scale)); new codes are
  * round(x * (1 / scale)), ties to even, saturated (NaN: 0).  Every step is a
  * correctly rounded fp32 operation (products and sums not contracted), so the bytes are reproducible.
+ * k, v and the cache's arrays do not overlap.
  * Appending the same rows twice gives the same cache as once.  A page that is appended to belongs to one
  * sequence, once: two that share it may only read it. */
 int htp_b200_kv_append(const struct HtpB200PagedKv *kv, const struct HtpB200Rope *rope, const void *k, int64_t k_stride,
@@ -315,7 +316,7 @@ int htp_b200_logits_process(float *dst, const float *src, int64_t stride, int ro
  * (0 = none), or -2 when the stream itself is in error.  The operators on a paged cache and on logits record
  * theirs per device, not per stream: 301 a page number out of range, 302 a sequence's row or context
  * lengths out of range, 303 a position outside the rotation table, 304 history or bias ranges, 305 a mask
- * row out of range; 311 a bounded wait inside the prompt attention ran out. */
+ * row out of range; 311 a bounded wait inside attention ran out. */
 int htp_b200_stream_status(void *stream);
 
 /* Tuning / debugging switches: "pdl" (programmatic dependent launch, default 1),

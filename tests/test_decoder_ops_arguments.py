@@ -48,6 +48,11 @@ def test_bad_appends(pkg, lib, change):
     assert append(pkg, lib, **change) == -1
 
 
+def test_appends_into_overlapping_arrays(pkg, lib):
+    assert append(pkg, lib, kv(pkg, v_codes=A + 16)) == -1 and append(pkg, lib, kv(pkg, v_scale=3 * A)) == -1
+    assert append(pkg, lib, k=A) == -1 and append(pkg, lib, v=2 * A + 1024) == -1
+
+
 @pytest.mark.parametrize("change", [dict(table=None), dict(table=A + 4), dict(table_len=0), dict(rot_dim=0), dict(rot_dim=12), dict(rot_dim=72), dict(mode=3), dict(mode=-1),
                                     dict(positions=A + 2)], ids=str)
 def test_bad_rotations(pkg, lib, change):

@@ -187,3 +187,71 @@ def test_captured_call_follows_the_lengths(pkg, lib):
         torch.cuda.synchronize()
         ref, mass, worst = dr.attention(c, q, 8, 0.1, 0)
         assert ((out.double().view_as(ref) - ref).abs() <= dr.attention_bound(ref, mass, worst, False, c.max_ctx)).all()
+
+
+@pytest.mark.parametrize("act", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_pages_behind_a_window_may_be_gone(pkg, lib, act, rows):
+    """Entries of pages that no row sees any more name nothing; nothing is reported and the rows are right."""
+    c = dr.Cache(pkg, [(rows, 700), (rows, 333)], page=16, heads=2, dim=64, kv="e4m3", seed=10)
+    q = torch.randn((2 * rows, 8 * 64), device="cuda").to(act)
+    ref, mass, worst = dr.attention(c, q, 8, 0.125, 50)
+    for b, (r, n) in enumerate(c.lens):
+        c.table[b, :(n - r + 1 - 50) // 16] = -7
+    out = torch.empty_like(q)
+    assert run(pkg, lib, c, q, 8, act, 0.125, 50, out) == 0
+    assert lib.htp_b200_stream_status(dr.stream()) == 0
+    assert ((out.double().view_as(ref) - ref).abs() <= dr.attention_bound(ref, mass, worst, act == torch.float32, c.max_ctx)).all()
+
+
+@pytest.mark.parametrize("act", [torch.float32, torch.float16], ids=["f32", "f16"])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_rows_do_not_see_each_other(pkg, lib, act, rows):
+    """NaN and infinities in some rows' queries leave the other rows as they are; a scale of 0 over codes of 0."""
+    c = dr.Cache(pkg, [(rows, 300), (rows, rows)], page=32, heads=2, dim=128, kv="i8", seed=11)
+    c.codes["v"][c.table[0, 2]], c.scale["v"][c.table[0, 2]] = 0, 0.0
+    c.codes["k"][c.table[0, 3]], c.scale["k"][c.table[0, 3]] = 0, 0.0
+    q = torch.randn((2 * rows, 6 * 128), device="cuda").to(act)
+    ref, mass, worst = dr.attention(c, q, 6, 0.1, 0)
+    q[1, 5] = float("nan")  # head 0
+    q[rows, 200] = float("inf")  # head 1
+    out = torch.empty_like(q)
+    assert run(pkg, lib, c, q, 6, act, 0.1, 0, out) == 0
+    got = out.double().view_as(ref)
+    keep = torch.ones_like(ref, dtype=torch.bool)
+    keep[1, 0] = keep[rows, 1] = False
+    bound = dr.attention_bound(ref, mass, worst, act == torch.float32, c.max_ctx)
+    assert ((got - ref).abs() <= bound)[keep].all()
+    assert torch.isnan(got[1, 0]).all()
+
+
+def test_bounds_of_a_call_above_what_it_has(pkg, lib):
+    """max_q and max_ctx as a captured program would give them, far above this step's rows and contexts."""
+    c = dr.Cache(pkg, [(1, 30), (3, 200), (1, 5)], page=16, heads=2, dim=64, kv="i8", seed=12, table_pad=600, extra_rows=60)
+    q = torch.randn((65, 4 * 64), device="cuda")
+    ref, mass, worst = dr.attention(c, q[:5], 4, 0.125, 0)
+    bound = dr.attention_bound(ref, mass, worst, True, c.max_ctx)
+    for max_q, max_ctx in ((3, 200), (3, 9000), (8, 9000), (64, 200), (64, 9000)):
+        ws = workspace_for(pkg, lib, c, 4, q.dtype, max_q, max_ctx)
+        for w in (ws, None):
+            out = torch.full_like(q, 3.0)
+            assert run(pkg, lib, c, q, 4, q.dtype, 0.125, 0, out, w, max_q, max_ctx) == 0
+            assert ((out[:5].double().view_as(ref) - ref).abs() <= bound).all() and (out[5:] == 3.0).all()
+    assert lib.htp_b200_stream_status(dr.stream()) == 0
+
+
+def test_calls_on_two_streams_at_once(pkg, lib):
+    """The same cache read by two streams, each with its own output and workspace, again and again."""
+    c = dr.Cache(pkg, [(1, 30000), (1, 700)], page=64, heads=1, dim=128, kv="e4m3", seed=13)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    qs = [torch.randn((2, 4 * 128), device="cuda").half() for _ in streams]
+    outs, wss = [torch.empty_like(q) for q in qs], [workspace_for(pkg, lib, c, 4, torch.float16) for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, q, out, ws in zip(streams, qs, outs, wss):
+            with torch.cuda.stream(s):
+                assert run(pkg, lib, c, q, 4, q.dtype, 0.1, 0, out, ws) == 0
+    torch.cuda.synchronize()
+    for q, out in zip(qs, outs):
+        ref, mass, worst = dr.attention(c, q, 4, 0.1, 0)
+        assert ((out.double().view_as(ref) - ref).abs() <= dr.attention_bound(ref, mass, worst, False, c.max_ctx)).all()
