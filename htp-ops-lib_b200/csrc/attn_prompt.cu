@@ -16,7 +16,10 @@
 // two fp16 terms each.  M follows the row's maximum only when it lags by more than kSlack, so O is rarely rescaled.
 //
 // Bound: per 128 x 128 scores 1024 cycles of tensor core at head_dim 128 and as many of the exponential unit
-// (16 per cycle and SM); fp32 doubles the tensor-core part.
+// (16 per cycle and SM); fp32 doubles the tensor-core part.  Measured: a prompt of 8192 rows, 32 + 8 heads of 128, fp16:
+// 643 us = 856 TF/s, 0.52 of the measured cuBLAS rate; per tile of two streams 4983 clocks, of which a stream's
+// softmax takes 2858, its wait for the next scores 1737 (the other stream's products, commits, the way through the
+// barriers), the MMA thread 2430.  6.5 k rows with a window of 1024, fp32: 388 us.
 //
 // Roles: warps 0-3 and 4-7 softmax of stream 0 and 1 (thread = row = TMEM lane), 8-11 converters, 12 MMA
 // issuer and tensor-memory owner, 13 scales.  All waits are bounded; one that runs out records error 311, raises the abort
