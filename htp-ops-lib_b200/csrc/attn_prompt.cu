@@ -43,6 +43,12 @@ constexpr int kThreads   = 14 * 32;
 constexpr int kKeys      = 128;  // keys of a tile
 constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more than a softmax warp may lag behind
 
+// The accumulator cuts off what lies below its last bit: sums come out short, on the average by about 1e-8 for each
+// instruction that a growing sum has gone through, 16 a tile with two terms (measured per tile: 1.6e-7 over 5 to 7 tiles,
+// 1.3e-7 over 28).  fp32 results get that back (prompts of 3300 keys: 1.6e-6 off without, 9.7e-7 with it); what fp16
+// results round away is a thousand times more.
+constexpr float kCut = 1.4e-7f;
+
 struct Bars {
   uint64_t q_full, k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_ready[2], o_done[2], drained;
   uint32_t tmem;
@@ -347,8 +353,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
           for (int h = 1; h < 4; ++h) {
             x0 = fmaxf(x0, fmaf(most[h], by[h], up[h]));
           }
-          // (first on a grid of 1 / 256, so that adding whole numbers is exact)
-          const float m = mx == kFloor ? fmaxf(ceilf(x0 * 256.f) * 0.00390625f, kFloor) : mx + fmaxf(ceilf(x0 - mx), 0.f);
+          // (first on a grid of 1 / 256, so that adding whole numbers is exact; never below the score, where a step is so
+          // large that it rounds)
+          const float m = mx == kFloor ? fmaxf(ceilf(x0 * 256.f) * 0.00390625f, kFloor) : fmaxf(mx + fmaxf(ceilf(x0 - mx), 0.f), x0);
           const int   k = __float2int_rn(fminf(m - mx, 127.f));
           const float f = __int_as_float((127 - k) << 23);  // (2^-127 and less: 0)
           mx = m;
@@ -459,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
 #pragma unroll
         for (int y = 0; y < (ROWS ? 1 : 2); ++y) {
           const int   z = ROWS ? x : y;
-          const float f = (y ? f1 : f0) * scale;
+          const float f = (y ? f1 : f0) * scale * (F32 ? fmaf((float) n_of[z], kCut, 1.f) : 1.f);
           if (n_of[z] > 0) {
             uint32_t o[32];
             tmem_ld32_issue(o_at(z) + lanes + 32 * c, o);
@@ -666,12 +673,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
       if (elect_one()) {
         const uint64_t kd = smem_desc_sw128(sK + i * TILE);
 #pragma unroll
-        for (int term = 0; term < TERMS; ++term) {
-          const uint64_t qd = smem_desc_sw128(sQ + (ROWS ? x : term) * TILE);
+        for (int i_ = 0; i_ < TERMS; ++i_) {  // (the small second term first: its sums lose nothing to the accumulator's steps)
+          const int      term = TERMS - 1 - i_;
+          const uint64_t qd   = smem_desc_sw128(sQ + (ROWS ? x : term) * TILE);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-            umma_f16_ss(s_at(x), qd + off, kd + off, IDESC_S, (term | k) ? 1u : 0u);
+            umma_f16_ss(s_at(x), qd + off, kd + off, IDESC_S, (i_ | k) ? 1u : 0u);
           }
         }
         umma_commit<false>(&bar->s_full[x]);

@@ -256,7 +256,8 @@ int htp_b200_kv_append(const struct HtpB200PagedKv *kv, const struct HtpB200Rope
  * sees: j <= its token number and, with window > 0, j > its token number - window; a row that sees none
  * gives zeros.  n_heads is a multiple of n_kv_heads, query head i reads key/value head
  * i / (n_heads / n_kv_heads).  out and q have act_type; fp32 queries and weights go through the
- * tensor cores as two fp16 terms each, so that fp32 results keep fp32 accuracy.
+ * tensor cores as two fp16 terms each, so that fp32 results keep fp32 accuracy (1e-6 of a row's size up to some
+ * thousand keys, 2e-6 for many rows over 8000).
  * max_q / max_ctx bound every sequence's rows / context in this call (a sequence over one of them is
  * skipped, error 302); they choose the kernel and its splits and do not change with the contents of a
  * captured call.  workspace: htp_b200_attn_workspace bytes of device memory, 16-byte aligned, contents of

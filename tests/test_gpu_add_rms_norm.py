@@ -9,6 +9,11 @@ import decoder_reference as dr
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(1)
+
+
 def statement(x, block, post, gate, weight, block_scale, eps):
     h = x.double()
     if block is not None:

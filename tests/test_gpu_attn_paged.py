@@ -9,6 +9,12 @@ import torch
 
 import decoder_reference as dr
 
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(1)
+
+
 pytestmark = pytest.mark.gpu
 
 SHAPES = [
@@ -91,12 +97,13 @@ def test_workspace_changes_nothing_but_the_split(pkg, lib, act):
 
 @pytest.mark.parametrize("act", [torch.float32, torch.float16], ids=["f32", "f16"])
 @pytest.mark.parametrize("rows", [1, 24])
-def test_scales_far_apart_and_peaked_scores(pkg, lib, act, rows):
+@pytest.mark.parametrize("seed", [0, 11, 13, 38])  # (0, 11, 38: scores that jump from moderate to huge within a row)
+def test_scales_far_apart_and_peaked_scores(pkg, lib, act, rows, seed):
     """Pages whose scales differ by many powers of two, scores up to some hundreds, large and tiny queries."""
     c = dr.Cache(pkg, [(rows, 400), (rows, 129)], page=16, heads=2, dim=64, kv="e4m3", seed=5, spread=4.0)
     c.scale["v"][0] = 2.0 ** -100  # (what the append gives a block of zeros)
     c.codes["v"][0] = 0
-    q = torch.randn((2 * rows, 4 * 64), device="cuda") * (100.0 if act == torch.float16 else 1.0)
+    q = torch.randn((2 * rows, 4 * 64), device="cuda", generator=torch.Generator("cuda").manual_seed(seed)) * (100.0 if act == torch.float16 else 1.0)
     if act == torch.float32:
         q[0] *= 3e5
         q[-1] *= 1e-6
@@ -105,8 +112,10 @@ def test_scales_far_apart_and_peaked_scores(pkg, lib, act, rows):
     assert run(pkg, lib, c, q, 4, act, 0.125, 0, out) == 0
     ref, mass, worst = dr.attention(c, q, 4, 0.125, 0)
     bound = dr.attention_bound(ref, mass, worst, act == torch.float32, c.max_ctx)
-    ok = (out.double().view_as(ref) - ref).abs() <= bound
-    assert ok.all()
+    got = out.double().view_as(ref)
+    if act == torch.float16:  # what lies above 65504 + 16 rounds to infinity: some of these values do
+        got = torch.where(got.isinf() & (ref.abs() + bound >= 65520) & (got.sign() == ref.sign()), ref, got)
+    assert ((got - ref).abs() <= bound).all()
 
 
 def test_bad_entries_are_skipped_and_reported(pkg, lib):

@@ -14,6 +14,11 @@ from test_gpu_logits import Case, close
 
 pytestmark = pytest.mark.gpu
 
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(1)
+
 HIDDEN, HEADS, KV_HEADS, DIM, VOCAB, PAGE = 512, 8, 2, 64, 1024, 16
 
 
