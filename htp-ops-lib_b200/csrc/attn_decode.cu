@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
       break;
     }
     // ---- scores
-    float s[2][NT][4];
+    float s[2][NT][4], s2[2][NT][4];  // (fp32: what the second terms make, apart: it is lost in no large sum)
     float by[2], up[2], inv[2];
     block_scales(scale[0][0], scale[0][1], a.scale_log2, by[0], up[0], inv[0]);  // (of the lane's tile)
 #pragma unroll
@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.f;
+        s2[m][n][0] = s2[m][n][1] = s2[m][n][2] = s2[m][n][3] = 0.f;
       }
     }
 #pragma unroll
@@ -321,9 +322,21 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const __grid_cons
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
               for (int x = 0; x < TERMS; ++x) {
-                mma_16816(s[m][n], af, w1 ? qf[n][x].z : qf[n][x].x, w1 ? qf[n][x].w : qf[n][x].y);
+                mma_16816(x ? s2[m][n] : s[m][n], af, w1 ? qf[n][x].z : qf[n][x].x, w1 ? qf[n][x].w : qf[n][x].y);
               }
             }
+          }
+        }
+      }
+    }
+    if constexpr (F32) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[m][n][e] += s2[m][n][e];
           }
         }
       }
