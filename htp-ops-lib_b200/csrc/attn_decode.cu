@@ -23,8 +23,8 @@
 // order; otherwise by independent CTAs whose results meet in the workspace and a second small launch
 // (attn_plan).  No atomics: results do not depend on scheduling.
 //
-// Bound: HBM; 64 contexts of up to 8192 tokens, fp16 and e4m3: 101 us for 539 MB = 0.81 of the measured copy rate (the
-// copies alone 85 us, the arithmetic alone 78); fp32 doubles the products: 2 contexts of 131072, 8 columns, 112 us.
+// Bound: HBM; 64 contexts of up to 8192 tokens, fp16 and e4m3: 97 us for 539 MB = 0.85 of the measured copy rate (the
+// copies alone 85 us, the arithmetic alone 78); fp32 doubles the products: 2 contexts of 131072, 8 columns, 114 us.
 #include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_fp16.h>

@@ -17,9 +17,9 @@
 //
 // Bound: per 128 x 128 scores 1024 cycles of tensor core at head_dim 128 and as many of the exponential unit
 // (16 per cycle and SM); fp32 doubles the tensor-core part.  Measured: a prompt of 8192 rows, 32 + 8 heads of 128, fp16:
-// 643 us = 856 TF/s, 0.52 of the measured cuBLAS rate; per tile of two streams 4983 clocks, of which a stream's
+// 643 us = 855 TF/s, 0.52 of the measured cuBLAS rate; per tile of two streams 4983 clocks, of which a stream's
 // softmax takes 2858, its wait for the next scores 1737 (the other stream's products, commits, the way through the
-// barriers), the MMA thread 2430.  6.5 k rows with a window of 1024, fp32: 388 us.
+// barriers), the MMA thread 2430.  6.5 k rows with a window of 1024, fp32: 376 us.
 //
 // Roles: warps 0-3 and 4-7 softmax of stream 0 and 1 (thread = row = TMEM lane), 8-11 converters, 12 MMA
 // issuer and tensor-memory owner, 13 scales.  All waits are bounded; one that runs out records error 311, raises the abort
@@ -45,7 +45,8 @@ constexpr int kScaleRing = 4;    // key tiles whose scales are kept: one more th
 
 // The accumulator cuts off what lies below its last bit: sums come out short, on the average by about 1e-8 for each
 // instruction that a growing sum has gone through, 16 a tile with two terms (measured per tile: 1.6e-7 over 5 to 7 tiles,
-// 1.3e-7 over 28).  fp32 results get that back (prompts of 3300 keys: 1.6e-6 off without, 9.7e-7 with it); what fp16
+// 1.3e-7 over 28).  fp32 results get that back (prompts of 3300 keys: 1.6e-6 off without, 9.7e-7 with it; three quarters of it where the
+// second terms have sums of their own); what fp16
 // results round away is a thousand times more.
 constexpr float kCut = 1.4e-7f;
 
@@ -104,6 +105,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
   static_assert(!(F32 && ROWS), "fp32 queries take the room of both row tiles");
   constexpr int TILE  = Sizes<D>::kTile;
   constexpr int TERMS = F32 ? 2 : 1;
+  // fp32 at head_dim 64: tensor memory has room to sum the second terms apart, in the columns behind O
+  constexpr int O2 = F32 && D == 64 ? 64 : 0;
   extern __shared__ uint8_t smem_raw[];
   // (an offset, not a rounded address: the compiler keeps seeing shared memory)
   uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int d = 0; d < D / 16; ++d) {
+        for (int d = 0; d < (D + O2) / 16; ++d) {
           tmem_ld16_issue(o_addr + 16 * d, w);
           tmem_ld_wait(w);
 #pragma unroll
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
 #pragma unroll
         for (int y = 0; y < (ROWS ? 1 : 2); ++y) {
           const int   z = ROWS ? x : y;
-          const float f = (y ? f1 : f0) * scale * (F32 ? fmaf((float) n_of[z], kCut, 1.f) : 1.f);
+          const float f = (y ? f1 : f0) * scale * (F32 ? fmaf((float) n_of[z], O2 ? 0.75f * kCut : kCut, 1.f) : 1.f);
           if (n_of[z] > 0) {
             uint32_t o[32];
             tmem_ld32_issue(o_at(z) + lanes + 32 * c, o);
@@ -474,6 +477,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               v[e] = fmaf(__uint_as_float(o[e]), f, v[e]);
+            }
+            if constexpr (O2 > 0) {
+              tmem_ld32_issue(o_at(z) + O2 + lanes + 32 * c, o);
+              tmem_ld_wait32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                v[e] = fmaf(__uint_as_float(o[e]), f, v[e]);
+              }
             }
           }
         }
@@ -716,8 +727,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prompt_kernel(const __grid_c
           for (int k = 0; k < kKeys / 16; ++k) {
 #pragma unroll
             for (int term = 0; term < TERMS; ++term) {
-              umma_f16_ts<false>(o_at(x), s_at(x) + 32 * (k >> 1) + 8 * (k & 1) + 16 * term, vd + k * (2048 >> 4), IDESC_O,
-                                 (j | k | term) ? 1u : 0u);
+              umma_f16_ts<false>(o_at(x) + O2 * term, s_at(x) + 32 * (k >> 1) + 8 * (k & 1) + 16 * term, vd + k * (2048 >> 4), IDESC_O,
+                                 (j | k | (O2 ? 0 : term)) ? 1u : 0u);
             }
           }
           umma_commit<false>(&bar->o_done[x]);
