@@ -264,3 +264,17 @@ def test_calls_on_two_streams_at_once(pkg, lib):
     for q, out in zip(qs, outs):
         ref, mass, worst = dr.attention(c, q, 4, 0.1, 0)
         assert ((out.double().view_as(ref) - ref).abs() <= dr.attention_bound(ref, mass, worst, False, c.max_ctx)).all()
+
+
+@pytest.mark.parametrize("heads", [2, 20])  # (the kernels for few and for many rows of a key/value head)
+def test_hundreds_of_sequences(pkg, lib, heads):
+    """More sequences than a CTA has threads, some of no rows, some of no tokens."""
+    c = dr.Cache(pkg, [(i % 3, i % 3 + (i * 7) % 50) for i in range(700)], page=16, heads=1, dim=64, kv="i8", seed=14, extra_rows=5)
+    n = c.starts[-1]
+    q = torch.randn((c.n_rows, heads * 64), device="cuda")
+    out = torch.full_like(q, 3.0)
+    assert run(pkg, lib, c, q, heads, torch.float32, 0.125, 0, out) == 0
+    assert lib.htp_b200_stream_status(dr.stream()) == 0
+    ref, mass, worst = dr.attention(c, q[:n], heads, 0.125, 0)
+    assert ((out[:n].double().view_as(ref) - ref).abs() <= dr.attention_bound(ref, mass, worst, True, c.max_ctx)).all()
+    assert (out[n:] == 3.0).all()

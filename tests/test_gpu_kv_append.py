@@ -149,3 +149,20 @@ def test_bad_entries_are_skipped_and_reported(pkg, lib):
     c.ctx_len[0] = 40
     attempt(0, False)
     same_cache(c, want)
+
+
+def test_hundreds_of_sequences(pkg, lib):
+    """More sequences than a CTA has threads, some of no rows."""
+    c = dr.Cache(pkg, [(i % 4, i % 4 + (i * 7) % 40) for i in range(600)], page=16, heads=1, dim=64, kv="e4m3", seed=7, extra_rows=3)
+    q, k, v = inputs(c, 2, torch.float32, 8)
+    table = angles(c.max_ctx, 32)
+    rope = pkg.Rope(table=table.data_ptr(), positions=None, table_len=len(table), rot_dim=32, mode=1)
+    want = dr.append(c, k, v, table, 32, 1)
+    q_out = torch.full((c.n_rows, 128), 3.0, device="cuda")
+    assert call(pkg, lib, c, k, v, q, q_out, 2, rope) == 0
+    assert lib.htp_b200_stream_status(dr.stream()) == 0
+    same_cache(c, want)
+    n = c.starts[-1]
+    pos = torch.cat([torch.arange(t - r, t, device="cuda") for r, t in c.lens])
+    assert torch.equal(q_out[:n].reshape(n, 2, 64), dr.rotate(q[:n].float().reshape(n, 2, 64), table[pos], 32, 1))
+    assert (q_out[n:] == 3.0).all()
